@@ -38,6 +38,9 @@ typedef enum uocr_quant_mode {
   UOCR_QUANT_NONE = 0,                /* BF16 weights, FP32 activations */
   UOCR_QUANT_WEIGHTS_ONLY = 1,        /* QuantizationMode::WeightsOnly */
   UOCR_QUANT_DYNAMIC_ACTIVATIONS = 2, /* QuantizationMode::DynamicActivations */
+  /* Vocabulary heads only; no counterpart in the reference: e4m3 weights with
+   * a scale per 128 x 128 tile, rows quantised per 128 columns. */
+  UOCR_QUANT_FP8_BLOCKS = 3,
 } uocr_quant_mode;
 
 /* Backend (src/cpu/mod.rs:10-16) with the GPU variant this library adds. */
@@ -48,6 +51,15 @@ typedef enum uocr_backend {
   UOCR_BACKEND_AUTO = 3,
   UOCR_BACKEND_GPU = 4,
 } uocr_backend;
+
+/* Safetensors dtypes (DType, src/checkpoint.rs:14-21). */
+typedef enum uocr_dtype {
+  UOCR_DTYPE_BF16 = 0,
+  UOCR_DTYPE_F16 = 1,
+  UOCR_DTYPE_F32 = 2,
+  UOCR_DTYPE_I64 = 3,
+  UOCR_DTYPE_I8 = 4,
+} uocr_dtype;
 
 /* Where the pointers handed to uocr_moe_layer_create live. */
 typedef enum uocr_memory {
@@ -323,6 +335,85 @@ int uocr_int8_linear_dynamic(uocr_gpu_ctx* ctx, const int8_t* q, const float* sc
 int uocr_rms_norm(uocr_gpu_ctx* ctx, const float* x, size_t rows, size_t width,
                   const float* weight, float eps, float* out);
 
+/* ------------------------------------- 8-bit floating point, token scores */
+/* No counterpart in the reference, whose quantised matrices are int8 with
+ * blocks of 32. Device pointers. Each operator has an _async form that is
+ * enqueued on the context stream and returns once queued (its device-side
+ * errors surface at uocr_gpu_ctx_synchronize; it launches kernels only, so it
+ * records into HIP graphs captured on the context stream) and a synchronous
+ * one. Inputs must be complete, and outputs free, in the order of the context
+ * stream. Operators that work in the context's scratch share it with the
+ * context's other calls: graphs captured on one context are not replayed at the
+ * same time.
+ *
+ * Values are e4m3 bytes (finite range +-448; 0x7f and 0xff are NaN). Blocks are
+ * 128 columns, the last of a row being shorter where cols is no multiple of
+ * 128. */
+#define UOCR_FP8_BLOCK 128
+/* Rows x[rows, cols] (BF16 or F32, row stride ld >= cols elements) to
+ * q[rows, cols] with scales[rows, ceil(cols / 128)]: x ~ q * scale. A scale is
+ * the least power of two that brings its block within +-448 (at least 2^-126; 1
+ * for a block of zeros), so x / scale is exact and q is its nearest e4m3, ties
+ * to even. A non-finite x -> Numerical. */
+int uocr_fp8_quantize(uocr_gpu_ctx* ctx, const void* x, uocr_dtype type, size_t rows, size_t cols,
+                      size_t ld, uint8_t* q, float* scales);
+int uocr_fp8_quantize_async(uocr_gpu_ctx* ctx, const void* x, uocr_dtype type, size_t rows,
+                            size_t cols, size_t ld, uint8_t* q, float* scales);
+/* A matrix, with one scale per 128 x 128 tile: scales[ceil(rows / 128),
+ * ceil(cols / 128)]; otherwise the same. Synchronous (weights are laid out
+ * once). */
+int uocr_fp8_quantize_weight(uocr_gpu_ctx* ctx, const void* w, uocr_dtype type, size_t rows,
+                             size_t cols, size_t ld, uint8_t* q, float* scales);
+/* y[m, n] = x . w^T of e4m3 rows x[m, k] with scales xs[m, ceil(k / 128)] and an
+ * e4m3 matrix w[n, k] with scales ws[ceil(n / 128), ceil(k / 128)]; any finite
+ * scales. Each block's products are summed and scaled in f32; y is F32 or BF16
+ * (rounded once). A NaN byte makes its row or column NaN and raises nothing.
+ * Equal calls give equal bits; a row's last bits depend on m, which chooses how
+ * its sums are split. */
+int uocr_fp8_linear(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
+                    const uint8_t* w, const float* ws, size_t n, void* y, uocr_dtype ytype);
+int uocr_fp8_linear_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
+                          const uint8_t* w, const float* ws, size_t n, void* y,
+                          uocr_dtype ytype);
+/* What to say of the distributions softmax(logits) of `rows` rows:
+ *   logprobs[rows]          log probability of tokens[row]
+ *   entropy[rows]           -sum p log p, in nats
+ *   top_ids, top_logprobs   [rows, n_top] the most probable ids in order of
+ *                           falling logit, equal ones by rising id
+ * tokens may be NULL where logprobs is; any output may be NULL (both top arrays
+ * where n_top is 0), not all. A negative token marks a padding row, which is not
+ * looked at: logprob and entropy 0, ids -1, alternatives' log probabilities
+ * -inf. n_top <= UOCR_MAX_TOP and <= the vocabulary.
+ * A logit of -inf is a banned id: probability 0. A row with a NaN or +inf, or
+ * with no finite logit, gets NaN (ids -1) and raises Numerical; a token at or
+ * past the vocabulary gets a NaN logprob and raises Shape. Statistics are held
+ * in f32. */
+#define UOCR_MAX_TOP 64
+typedef struct uocr_token_scores {
+  const int32_t* tokens; /* [rows] */
+  size_t n_top;
+  float* logprobs;
+  float* entropy;
+  int32_t* top_ids;
+  float* top_logprobs;
+} uocr_token_scores;
+/* Scores of logits[rows, vocab] in memory (BF16, F16 or F32, row stride ld >=
+ * vocab elements). */
+int uocr_token_logprobs(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype type, size_t rows,
+                        size_t vocab, size_t ld, const uocr_token_scores* scores);
+int uocr_token_logprobs_async(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype type, size_t rows,
+                              size_t vocab, size_t ld, const uocr_token_scores* scores);
+/* Scores of the rows of uocr_fp8_linear's product. With n_top 0 the logits stay
+ * in registers (scratch: some 16 bytes per row and 256 ids); alternatives take
+ * them through the context's scratch in f32, as many rows at a time as fit
+ * (none: Resource). A logit that is not finite raises Numerical. */
+int uocr_fp8_linear_logprobs(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m,
+                             size_t k, const uint8_t* w, const float* ws, size_t n,
+                             const uocr_token_scores* scores);
+int uocr_fp8_linear_logprobs_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m,
+                                   size_t k, const uint8_t* w, const float* ws, size_t n,
+                                   const uocr_token_scores* scores);
+
 /* ------------------------------------------------- vocabulary projection */
 /* Decoder::logits (src/decoder/mod.rs:367-379): the last hidden row,
  * RMSNorm with model.norm.weight, then Decoder::projection (:99-112) with
@@ -336,8 +427,10 @@ typedef struct uocr_lm_head_weights {
   float rms_norm_eps;
   const float* norm_weight;  /* model.norm.weight widened to f32, [H] */
   const uint16_t* weight;    /* lm_head.weight bf16 bits [V, H]; may be NULL with q */
-  const int8_t* q;           /* overlay lm_head.weight [V, H], or NULL */
-  const float* scales;       /* its .q8_scales [V, H/32] */
+  const int8_t* q;           /* overlay lm_head.weight [V, H], or NULL; e4m3
+                              * bytes under UOCR_QUANT_FP8_BLOCKS */
+  const float* scales;       /* its .q8_scales [V, H/32]; under
+                              * UOCR_QUANT_FP8_BLOCKS [ceil(V/128), ceil(H/128)] */
   uocr_quant_mode quant_mode; /* UOCR_QUANT_NONE when q is NULL */
 } uocr_lm_head_weights;
 int uocr_lm_head_create(uocr_gpu_ctx* ctx, const uocr_lm_head_weights* w, uocr_memory where,
@@ -348,7 +441,19 @@ int uocr_lm_head_logits(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float
                         size_t T, float* logits);
 int uocr_lm_head_logits_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,
                               size_t T, float* logits);
-/* "bf16_weights_fp32", "int8_weights_fp32", "int8_weights_dynamic_activations". */
+/* Scores of the tokens that follow each of hidden[T, H]'s rows (all of them, not
+ * the last one only): RMSNorm, the projection, then uocr_token_scores over the
+ * vocabulary. Multi-row projections follow Decoder::projection: INT8 weights
+ * with FP32 rows (W8A8 only where T == 1 under DynamicActivations). FP8 heads
+ * quantise each normalised row and score it as uocr_fp8_linear_logprobs does;
+ * the others hold logits in the context's scratch, as many rows at a time as
+ * fit. T == 0 is a no-op. */
+int uocr_lm_head_logprobs(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,
+                          size_t T, const uocr_token_scores* scores);
+int uocr_lm_head_logprobs_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,
+                                size_t T, const uocr_token_scores* scores);
+/* "bf16_weights_fp32", "int8_weights_fp32", "int8_weights_dynamic_activations",
+ * "fp8_weights_dynamic_activations". */
 const char* uocr_lm_head_precision(const uocr_lm_head* head);
 size_t uocr_lm_head_device_bytes(const uocr_lm_head* head);
 void uocr_lm_head_destroy(uocr_lm_head* head);
@@ -356,15 +461,6 @@ void uocr_lm_head_destroy(uocr_lm_head* head);
 /* ---------------------------------------------------- checkpoint files */
 /* The model-directory side of Model::load_with_quantization; the C++ form
  * of each is in uocr.hpp. */
-
-/* Safetensors dtypes (DType, src/checkpoint.rs:14-21). */
-typedef enum uocr_dtype {
-  UOCR_DTYPE_BF16 = 0,
-  UOCR_DTYPE_F16 = 1,
-  UOCR_DTYPE_F32 = 2,
-  UOCR_DTYPE_I64 = 3,
-  UOCR_DTYPE_I8 = 4,
-} uocr_dtype;
 
 typedef struct uocr_checkpoint uocr_checkpoint;
 /* Checkpoint::open (src/checkpoint.rs:114-178): memory-maps a safetensors

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../include/uocr_moe.h"
+#include "fp8.hpp"
 #include "moe_kernels.hpp"
 
 using uocr::DeviceLayer;
@@ -354,6 +355,7 @@ int read_and_clear_error(uocr_gpu_ctx* ctx) {
             "reset the decode partials");
     HIP_TRY(hipStreamSynchronize(ctx->stream), "synchronize");
     return fail(e, e == UOCR_ERR_NUMERICAL  ? "nonfinite numerical input on device"
+                   : e == UOCR_ERR_SHAPE     ? "token id outside the vocabulary"
                    : e == UOCR_ERR_RESOURCE ? "a one-token launch's cross-workgroup wait reached its bound"
                                             : "device reported an error");
   }
@@ -1253,6 +1255,226 @@ int uocr_rms_norm(uocr_gpu_ctx* ctx, const float* x, size_t rows, size_t width,
 }
 
 
+// -------------------------------------- 8-bit floating point, token scores
+
+}  // extern "C"
+
+namespace {
+
+static_assert(UOCR_FP8_BLOCK == uocr::kFp8Block && UOCR_MAX_TOP == uocr::kMaxTop, "header constants");
+static_assert(UOCR_DTYPE_BF16 == uocr::kTypeBf16 && UOCR_DTYPE_F16 == uocr::kTypeF16 &&
+                  UOCR_DTYPE_F32 == uocr::kTypeF32,
+              "element types");
+
+// Largest extents of one call: launches hold fewer than 2^32 threads, and a
+// tile's byte range (256 rows of k) stays below 2^31.
+constexpr size_t kMostRows = (size_t)1 << 22, kMostCols = (size_t)1 << 22;
+
+size_t fp8_blocks(size_t n) { return (n + UOCR_FP8_BLOCK - 1) / UOCR_FP8_BLOCK; }
+
+int check_quantize(uocr_gpu_ctx* ctx, const void* x, uocr_dtype type, size_t rows, size_t cols,
+                   size_t ld, uint8_t* q, float* scales) {
+  if (!ctx) return fail(UOCR_ERR_SHAPE, "null context");
+  if (type != UOCR_DTYPE_BF16 && type != UOCR_DTYPE_F32)
+    return fail(UOCR_ERR_UNSUPPORTED, "rows to quantise are BF16 or F32");
+  if (cols == 0 || ld < cols) return fail(UOCR_ERR_SHAPE, "rows must be [rows, cols], stride >= cols");
+  if (rows && (!x || !q || !scales)) return fail(UOCR_ERR_SHAPE, "null pointer");
+  if (rows > kMostRows || cols > kMostCols || rows * fp8_blocks(cols) >= (size_t)1 << 28)
+    return fail(UOCR_ERR_RESOURCE, "too many rows or columns for one call");
+  return UOCR_OK;
+}
+
+int check_product(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
+                  const uint8_t* w, const float* ws, size_t n) {
+  if (!ctx) return fail(UOCR_ERR_SHAPE, "null context");
+  if (k == 0 || n == 0) return fail(UOCR_ERR_SHAPE, "linear weight must be [out,in]");
+  if (m && (!x || !xs || !w || !ws)) return fail(UOCR_ERR_SHAPE, "null pointer");
+  if (m > kMostRows || n > kMostRows || k > kMostCols || fp8_blocks(m) * fp8_blocks(n) >= (size_t)1 << 24)
+    return fail(UOCR_ERR_RESOURCE, "too many rows or columns for one call");
+  return UOCR_OK;
+}
+
+int check_scores(const uocr_token_scores* s, size_t rows, size_t vocab) {
+  if (!s) return fail(UOCR_ERR_SHAPE, "missing scores");
+  if (s->logprobs && !s->tokens && rows)
+    return fail(UOCR_ERR_SHAPE, "log probabilities need the given tokens");
+  if (s->n_top > vocab) return fail(UOCR_ERR_SHAPE, "more alternatives than ids");
+  if (s->n_top > UOCR_MAX_TOP)
+    return fail(UOCR_ERR_UNSUPPORTED, "at most %d alternatives", UOCR_MAX_TOP);
+  if (rows && s->n_top && (!s->top_ids || !s->top_logprobs))
+    return fail(UOCR_ERR_SHAPE, "alternatives need both of their arrays");
+  if (rows && !s->n_top && !s->logprobs && !s->entropy)
+    return fail(UOCR_ERR_SHAPE, "no score is asked for");
+  return UOCR_OK;
+}
+
+uocr::TokenScores scores_from(const uocr_token_scores& s, size_t row) {
+  uocr::TokenScores o;
+  o.top = (int)s.n_top;
+  o.tokens = s.tokens ? s.tokens + row : nullptr;
+  o.logprobs = s.logprobs ? s.logprobs + row : nullptr;
+  o.entropy = s.entropy ? s.entropy + row : nullptr;
+  o.top_ids = s.n_top ? s.top_ids + row * s.n_top : nullptr;
+  o.top_logprobs = s.n_top ? s.top_logprobs + row * s.n_top : nullptr;
+  return o;
+}
+
+// The most rows, at most m, whose need(rows) bytes fit (0: not even one).
+template <class Need>
+size_t rows_that_fit(size_t m, size_t limit, const Need& need) {
+  size_t rows = m;
+  while (rows && need(rows) > limit) rows = rows == 1 ? 0 : (rows + 1) / 2;
+  return rows;
+}
+
+int scratch_fail(uocr_gpu_ctx* ctx) {
+  return fail(UOCR_ERR_RESOURCE, "operation exceeds scratch limit (%zu bytes)", ctx->scratch_limit);
+}
+
+// Bytes of score work for `rows` rows of logits or of a product; n_top > 0
+// brings the product's logits into scratch too.
+size_t logits_need(size_t rows, size_t vocab, const uocr_token_scores& s) {
+  return align256(rows * vocab * 4) +
+         align256(uocr::token_score_bytes(rows, (int)vocab, uocr::kTypeF32, (int)s.n_top));
+}
+size_t product_need(const uocr::Fp8Product& p, size_t rows, const uocr_token_scores& s) {
+  uocr::Fp8Product q = p;
+  q.m = (int)rows;
+  return s.n_top ? logits_need(rows, p.n, s) : align256(uocr::fp8_score_bytes(q));
+}
+
+// Scores rows [row, row + p.m) of the caller's arrays from the product p, in
+// the scratch at `work` (product_need bytes).
+void enqueue_product_scores(uocr_gpu_ctx* ctx, const uocr::Fp8Product& p, char* work,
+                            const uocr_token_scores& s, size_t row) {
+  const uocr::TokenScores o = scores_from(s, row);
+  if (s.n_top) {
+    uocr::launch_fp8_linear(p, work, uocr::kTypeF32, ctx->stream);
+    uocr::launch_token_scores(work, uocr::kTypeF32, p.m, p.n, p.n, o,
+                              work + align256((size_t)p.m * p.n * 4), ctx->err, ctx->stream);
+  } else {
+    uocr::launch_fp8_scores(p, o, work, ctx->err, ctx->stream);
+  }
+}
+
+// e4m3 bytes without NaN, finite nonnegative scales.
+__global__ void check_fp8_kernel(const uint8_t* q, size_t nq, const float* s, size_t ns, int* flag) {
+  const size_t stride = (size_t)gridDim.x * blockDim.x, at = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+  for (size_t i = at; i < nq; i += stride)
+    if ((q[i] & 0x7f) == 0x7f) atomicMax(flag, UOCR_ERR_FORMAT);
+  for (size_t i = at; i < ns; i += stride)
+    if (!isfinite(s[i]) || s[i] < 0.f) atomicMax(flag, UOCR_ERR_NUMERICAL);
+}
+
+}  // namespace
+
+extern "C" {
+
+int uocr_fp8_quantize_async(uocr_gpu_ctx* ctx, const void* x, uocr_dtype type, size_t rows,
+                            size_t cols, size_t ld, uint8_t* q, float* scales) {
+  if (int r = check_quantize(ctx, x, type, rows, cols, ld, q, scales)) return r;
+  if (rows == 0) return UOCR_OK;
+  HIP_TRY(hipSetDevice(ctx->device), "set device");
+  uocr::launch_fp8_quantize(x, type, rows, (int)cols, ld, q, scales, ctx->err, ctx->stream);
+  HIP_TRY(hipGetLastError(), "kernel launch");
+  return UOCR_OK;
+}
+
+int uocr_fp8_quantize(uocr_gpu_ctx* ctx, const void* x, uocr_dtype type, size_t rows, size_t cols,
+                      size_t ld, uint8_t* q, float* scales) {
+  const int r = uocr_fp8_quantize_async(ctx, x, type, rows, cols, ld, q, scales);
+  return r || rows == 0 ? r : read_and_clear_error(ctx);
+}
+
+int uocr_fp8_quantize_weight(uocr_gpu_ctx* ctx, const void* w, uocr_dtype type, size_t rows,
+                             size_t cols, size_t ld, uint8_t* q, float* scales) {
+  if (int r = check_quantize(ctx, w, type, rows, cols, ld, q, scales)) return r;
+  if (rows == 0) return UOCR_OK;
+  HIP_TRY(hipSetDevice(ctx->device), "set device");
+  uocr::launch_fp8_quantize_tiles(w, type, (int)rows, (int)cols, ld, q, scales, ctx->err, ctx->stream);
+  HIP_TRY(hipGetLastError(), "kernel launch");
+  return read_and_clear_error(ctx);
+}
+
+int uocr_fp8_linear_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
+                          const uint8_t* w, const float* ws, size_t n, void* y, uocr_dtype ytype) {
+  if (int r = check_product(ctx, x, xs, m, k, w, ws, n)) return r;
+  if (ytype != UOCR_DTYPE_BF16 && ytype != UOCR_DTYPE_F32)
+    return fail(UOCR_ERR_UNSUPPORTED, "products are BF16 or F32");
+  if (m == 0) return UOCR_OK;
+  if (!y) return fail(UOCR_ERR_SHAPE, "null pointer");
+  HIP_TRY(hipSetDevice(ctx->device), "set device");
+  uocr::launch_fp8_linear({x, xs, w, ws, (int)m, (int)n, (int)k}, y, ytype, ctx->stream);
+  HIP_TRY(hipGetLastError(), "kernel launch");
+  return UOCR_OK;
+}
+
+int uocr_fp8_linear(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
+                    const uint8_t* w, const float* ws, size_t n, void* y, uocr_dtype ytype) {
+  const int r = uocr_fp8_linear_async(ctx, x, xs, m, k, w, ws, n, y, ytype);
+  return r || m == 0 ? r : read_and_clear_error(ctx);
+}
+
+int uocr_token_logprobs_async(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype type, size_t rows,
+                              size_t vocab, size_t ld, const uocr_token_scores* scores) {
+  if (!ctx) return fail(UOCR_ERR_SHAPE, "null context");
+  if (type != UOCR_DTYPE_BF16 && type != UOCR_DTYPE_F16 && type != UOCR_DTYPE_F32)
+    return fail(UOCR_ERR_UNSUPPORTED, "logits are BF16, F16 or F32");
+  if (vocab == 0 || ld < vocab) return fail(UOCR_ERR_SHAPE, "logits must be [rows, vocab], stride >= vocab");
+  if (int r = check_scores(scores, rows, vocab)) return r;
+  if (rows == 0) return UOCR_OK;
+  if (!logits) return fail(UOCR_ERR_SHAPE, "null pointer");
+  if (rows > kMostRows || vocab > (size_t)INT32_MAX / 2)
+    return fail(UOCR_ERR_RESOURCE, "too many rows or ids for one call");
+  HIP_TRY(hipSetDevice(ctx->device), "set device");
+  auto need = [&](size_t r) { return uocr::token_score_bytes(r, (int)vocab, type, (int)scores->n_top); };
+  const size_t fit = rows_that_fit(rows, ctx->scratch_limit, need);
+  if (!fit) return scratch_fail(ctx);
+  const size_t step = std::min(fit, uocr::token_score_rows((int)vocab, type));
+  for (size_t r = 0; r < rows; r += step) {
+    uocr::launch_token_scores(static_cast<const char*>(logits) + r * ld * (type == UOCR_DTYPE_F32 ? 4 : 2),
+                              type, std::min(step, rows - r), (int)vocab, ld, scores_from(*scores, r),
+                              ctx->scratch, ctx->err, ctx->stream);
+    HIP_TRY(hipGetLastError(), "kernel launch");
+  }
+  return UOCR_OK;
+}
+
+int uocr_token_logprobs(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype type, size_t rows,
+                        size_t vocab, size_t ld, const uocr_token_scores* scores) {
+  const int r = uocr_token_logprobs_async(ctx, logits, type, rows, vocab, ld, scores);
+  return r || rows == 0 ? r : read_and_clear_error(ctx);
+}
+
+int uocr_fp8_linear_logprobs_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m,
+                                   size_t k, const uint8_t* w, const float* ws, size_t n,
+                                   const uocr_token_scores* scores) {
+  if (int r = check_product(ctx, x, xs, m, k, w, ws, n)) return r;
+  if (int r = check_scores(scores, m, n)) return r;
+  if (m == 0) return UOCR_OK;
+  HIP_TRY(hipSetDevice(ctx->device), "set device");
+  uocr::Fp8Product p{x, xs, w, ws, (int)m, (int)n, (int)k};
+  const size_t step = std::min(
+      rows_that_fit(m, ctx->scratch_limit, [&](size_t r) { return product_need(p, r, *scores); }),
+      uocr::token_score_rows((int)n, uocr::kTypeF32));
+  if (!step) return scratch_fail(ctx);
+  for (size_t r = 0; r < m; r += step) {
+    p.x = x + r * k;
+    p.xs = xs + r * p.kblocks();
+    p.m = (int)std::min(step, m - r);
+    enqueue_product_scores(ctx, p, ctx->scratch, *scores, r);
+    HIP_TRY(hipGetLastError(), "kernel launch");
+  }
+  return UOCR_OK;
+}
+
+int uocr_fp8_linear_logprobs(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m,
+                             size_t k, const uint8_t* w, const float* ws, size_t n,
+                             const uocr_token_scores* scores) {
+  const int r = uocr_fp8_linear_logprobs_async(ctx, x, xs, m, k, w, ws, n, scores);
+  return r || m == 0 ? r : read_and_clear_error(ctx);
+}
+
 // ------------------------------------------------- vocabulary projection
 
 int uocr_lm_head_create(uocr_gpu_ctx* ctx, const uocr_lm_head_weights* w, uocr_memory where,
@@ -1266,7 +1488,10 @@ int uocr_lm_head_create(uocr_gpu_ctx* ctx, const uocr_lm_head_weights* w, uocr_m
   if (!std::isfinite(w->rms_norm_eps) || w->rms_norm_eps <= 0.f)
     return fail(UOCR_ERR_SHAPE, "invalid normalization parameters");
   const bool quant = w->q != nullptr;
-  if (quant) {
+  const bool fp8 = quant && w->quant_mode == UOCR_QUANT_FP8_BLOCKS;
+  if (fp8) {
+    if (!w->scales) return fail(UOCR_ERR_FORMAT, "missing lm_head.weight scales");
+  } else if (quant) {
     if (w->quant_mode != UOCR_QUANT_WEIGHTS_ONLY && w->quant_mode != UOCR_QUANT_DYNAMIC_ACTIVATIONS)
       return fail(UOCR_ERR_SHAPE, "an INT8 lm_head needs a quantization mode");
     if (!w->scales) return fail(UOCR_ERR_FORMAT, "missing lm_head.weight.q8_scales");
@@ -1282,7 +1507,7 @@ int uocr_lm_head_create(uocr_gpu_ctx* ctx, const uocr_lm_head_weights* w, uocr_m
   head->view.V = (int)V;
   head->view.H = (int)H;
   head->view.eps = w->rms_norm_eps;
-  head->view.kind = !quant ? 0 : (w->quant_mode == UOCR_QUANT_DYNAMIC_ACTIVATIONS ? 2 : 1);
+  head->view.kind = !quant ? 0 : fp8 ? 3 : (w->quant_mode == UOCR_QUANT_DYNAMIC_ACTIVATIONS ? 2 : 1);
   auto finish = [&](int status) {
     if (status) uocr_lm_head_destroy(head);
     return status;
@@ -1303,8 +1528,17 @@ int uocr_lm_head_create(uocr_gpu_ctx* ctx, const uocr_lm_head_weights* w, uocr_m
   if (quant) {
     if ((r = alloc_copy(w->q, V * H, &p))) return finish(r);
     head->view.q = static_cast<const int8_t*>(p);
-    if ((r = alloc_copy(w->scales, V * (H / 32) * 4, &p))) return finish(r);
+    const size_t scales = fp8 ? fp8_blocks(V) * fp8_blocks(H) : V * (H / 32);
+    if ((r = alloc_copy(w->scales, scales * 4, &p))) return finish(r);
     head->view.s = static_cast<const float*>(p);
+    if (fp8) {
+      if ((r = read_and_clear_error(ctx))) return finish(r);  // of earlier calls
+      check_fp8_kernel<<<1024, 256, 0, ctx->stream>>>(reinterpret_cast<const uint8_t*>(head->view.q), V * H,
+                                                      head->view.s, scales, ctx->err);
+      if ((r = read_and_clear_error(ctx)))
+        return finish(fail(r, r == UOCR_ERR_FORMAT ? "invalid e4m3 matrix (NaN byte)"
+                                                   : "scales must be finite and nonnegative"));
+    }
   } else {
     if ((r = alloc_copy(w->weight, V * H * 2, &p))) return finish(r);
     head->view.w = static_cast<const uint16_t*>(p);
@@ -1313,6 +1547,54 @@ int uocr_lm_head_create(uocr_gpu_ctx* ctx, const uocr_lm_head_weights* w, uocr_m
   *out = head;
   return UOCR_OK;
 }
+
+}  // extern "C"
+
+namespace {
+
+// Normalised rows of a head's input in scratch: f32, and for FP8 heads e4m3
+// with their scales.
+struct HeadRows {
+  float* xn;
+  uint8_t* q;
+  float* xs;
+  size_t bytes;
+};
+HeadRows head_rows(char* base, const uocr::LmHeadView& v, size_t rows) {
+  HeadRows h{};
+  h.xn = reinterpret_cast<float*>(base);
+  h.bytes = align256(rows * v.H * 4);
+  if (v.kind == 3) {
+    h.q = reinterpret_cast<uint8_t*>(base + h.bytes);
+    h.bytes += align256(rows * v.H);
+    h.xs = reinterpret_cast<float*>(base + h.bytes);
+    h.bytes += align256(rows * fp8_blocks(v.H) * 4);
+  }
+  return h;
+}
+
+void normalized_head_rows(uocr_gpu_ctx* ctx, const uocr::LmHeadView& v, const float* hidden,
+                          size_t rows, const HeadRows& h) {
+  uocr::RowNorm nn;
+  nn.w = v.norm_w;
+  nn.eps = v.eps;
+  nn.out = h.xn;
+  uocr::launch_rms_norm(hidden, (int)rows, v.H, nn, ctx->err, ctx->stream);
+}
+
+void quantized_head_rows(uocr_gpu_ctx* ctx, const uocr::LmHeadView& v, const float* hidden,
+                         size_t rows, const HeadRows& h) {
+  normalized_head_rows(ctx, v, hidden, rows, h);
+  uocr::launch_fp8_quantize(h.xn, uocr::kTypeF32, rows, v.H, v.H, h.q, h.xs, ctx->err, ctx->stream);
+}
+
+uocr::Fp8Product fp8_head(const uocr::LmHeadView& v, const HeadRows& h, size_t rows) {
+  return {h.q, h.xs, reinterpret_cast<const uint8_t*>(v.q), v.s, (int)rows, v.V, v.H};
+}
+
+}  // namespace
+
+extern "C" {
 
 int uocr_lm_head_logits_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,
                               size_t T, float* logits) {
@@ -1323,7 +1605,12 @@ int uocr_lm_head_logits_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const
   HIP_TRY(hipSetDevice(ctx->device), "set device");
   const uocr::LmHeadView& v = head->view;
   const float* last = hidden + (T - 1) * (size_t)v.H;
-  if (uocr::lm_head_fast(v.H)) {
+  if (v.kind == 3) {
+    const HeadRows rows = head_rows(ctx->scratch, v, 1);
+    if (rows.bytes > ctx->scratch_limit) return scratch_fail(ctx);
+    quantized_head_rows(ctx, v, last, 1, rows);
+    uocr::launch_fp8_linear(fp8_head(v, rows, 1), logits, uocr::kTypeF32, ctx->stream);
+  } else if (uocr::lm_head_fast(v.H)) {
     uocr::launch_lm_head(last, v, logits, ctx->err, ctx->stream);
   } else {
     // Other widths: the norm into scratch, then the single-matrix operators.
@@ -1358,11 +1645,71 @@ int uocr_lm_head_logits(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float
   return read_and_clear_error(ctx);
 }
 
+int uocr_lm_head_logprobs_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,
+                                size_t T, const uocr_token_scores* scores) {
+  if (!ctx || !head) return fail(UOCR_ERR_SHAPE, "null handle");
+  const uocr::LmHeadView& v = head->view;
+  if (int r = check_scores(scores, T, v.V)) return r;
+  if (T == 0) return UOCR_OK;
+  if (!hidden) return fail(UOCR_ERR_SHAPE, "null hidden rows");
+  if (T > kMostRows) return fail(UOCR_ERR_RESOURCE, "too many rows for one call");
+  if (head->device != ctx->device) return fail(UOCR_ERR_SHAPE, "lm_head lives on another device");
+  HIP_TRY(hipSetDevice(ctx->device), "set device");
+  const size_t V = (size_t)v.V, H = (size_t)v.H;
+  const bool fp8 = v.kind == 3;
+  // One row under DynamicActivations is projected W8A8, from a quantised copy.
+  const bool w8a8 = v.kind == 2 && T == 1;
+  const size_t row8 = w8a8 ? align256(H) + align256((H + 31) / 32 * 4) : 0;
+  auto need = [&](size_t rows) {
+    const size_t head_bytes = head_rows(nullptr, v, rows).bytes;
+    return head_bytes + row8 + (fp8 ? product_need(fp8_head(v, {}, rows), rows, *scores)
+                                    : logits_need(rows, V, *scores));
+  };
+  const size_t step = std::min(rows_that_fit(T, ctx->scratch_limit, need),
+                               uocr::token_score_rows(v.V, uocr::kTypeF32));
+  if (!step) return scratch_fail(ctx);
+  for (size_t t = 0; t < T; t += step) {
+    const size_t rows = std::min(step, T - t);
+    const float* in = hidden + t * H;
+    const HeadRows h = head_rows(ctx->scratch, v, rows);
+    char* work = ctx->scratch + h.bytes;
+    if (fp8) {
+      quantized_head_rows(ctx, v, in, rows, h);
+      enqueue_product_scores(ctx, fp8_head(v, h, rows), work, *scores, t);
+    } else {
+      float* logits = reinterpret_cast<float*>(work);
+      char* after = work + align256(rows * V * 4);
+      normalized_head_rows(ctx, v, in, rows, h);
+      if (v.kind == 0) {
+        uocr::launch_linear_bf16(h.xn, (int)rows, v.H, v.w, v.V, logits, ctx->stream);
+      } else if (w8a8) {
+        uocr::launch_int8_dynamic(v.q, v.s, v.V, v.H, h.xn, logits, nullptr,
+                                  reinterpret_cast<int8_t*>(after),
+                                  reinterpret_cast<float*>(after + align256(H)), ctx->err, ctx->stream);
+        after += row8;
+      } else {
+        uocr::launch_int8_linear(v.q, v.s, v.V, v.H, h.xn, (int)rows, logits, ctx->stream);
+      }
+      uocr::launch_token_scores(logits, uocr::kTypeF32, rows, v.V, V, scores_from(*scores, t), after,
+                                ctx->err, ctx->stream);
+    }
+    HIP_TRY(hipGetLastError(), "kernel launch");
+  }
+  return UOCR_OK;
+}
+
+int uocr_lm_head_logprobs(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,
+                          size_t T, const uocr_token_scores* scores) {
+  const int r = uocr_lm_head_logprobs_async(ctx, head, hidden, T, scores);
+  return r || T == 0 ? r : read_and_clear_error(ctx);
+}
+
 const char* uocr_lm_head_precision(const uocr_lm_head* head) {
   if (!head) return "";
   return head->view.kind == 0   ? "bf16_weights_fp32"
          : head->view.kind == 1 ? "int8_weights_fp32"
-                                : "int8_weights_dynamic_activations";
+         : head->view.kind == 2 ? "int8_weights_dynamic_activations"
+                                : "fp8_weights_dynamic_activations";
 }
 
 size_t uocr_lm_head_device_bytes(const uocr_lm_head* head) { return head ? head->bytes : 0; }

@@ -1,0 +1,419 @@
+// 8-bit floating point (e4m3) with a scale per block of 128: rows quantised,
+// and the product of such rows with a matrix of 128 x 128 tiles.
+//
+//   y[i][j] = sum_b xs[i][b] ws[j / 128][b] sum_{k in block b} x[i][k] w[j][k]
+//
+// No counterpart in the reference, whose overlay is int8 with blocks of 32
+// (src/cpu/quantized.rs:9-237); these stand beside its operators.
+#include "fp8.hpp"
+#include "mfma.hpp"
+#include "scores.hpp"
+
+namespace uocr {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------- quantisation
+
+// The scale of a block whose largest magnitude has the bits `most`: the least
+// power of two s with most / s <= 448 = 1.75 * 2^8, at least 2^-126; 1 for a
+// block of zeros. As biased exponents; a power of two makes x / s exact, so the
+// only rounding is the one to e4m3, and costs nothing against most / 448: the
+// relative step of a floating format does not depend on the scale.
+__device__ __forceinline__ uint32_t scale_exponent(uint32_t most) {
+  if (most == 0) return 127;
+  const int e = (int)(most >> 23) - 8 + ((most & 0x7fffffu) > 0x600000u);
+  return (uint32_t)max(e, 1);
+}
+
+template <typename T>
+__device__ __forceinline__ float widen(T v);
+template <>
+__device__ __forceinline__ float widen<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ float widen<uint16_t>(uint16_t v) {
+  return __uint_as_float((uint32_t)v << 16);
+}
+
+__device__ __forceinline__ uint32_t max_u32(uint32_t a, uint32_t b) { return a > b ? a : b; }
+
+// Eight values of one lane as e4m3 (round to nearest even), two words.
+__device__ __forceinline__ uint2 to_fp8x8(const float (&v)[8], float inverse) {
+  int lo = 0, hi = 0;
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inverse, v[1] * inverse, lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inverse, v[3] * inverse, lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4] * inverse, v[5] * inverse, hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6] * inverse, v[7] * inverse, hi, true);
+  return make_uint2((uint32_t)lo, (uint32_t)hi);
+}
+
+// Eight consecutive elements at p, of which `have` exist (zeros behind them).
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T* p, int have, float (&v)[8]) {
+  if (WIDE) {
+    if (have > 0) {
+      if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0];
+        const float4 b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        v[0] = bf16_lo(a.x), v[1] = bf16_hi(a.x), v[2] = bf16_lo(a.y), v[3] = bf16_hi(a.y);
+        v[4] = bf16_lo(a.z), v[5] = bf16_hi(a.z), v[6] = bf16_lo(a.w), v[7] = bf16_hi(a.w);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = j < have ? widen<T>(p[j]) : 0.0f;
+  }
+}
+
+template <bool WIDE>
+__device__ __forceinline__ void store8(uint8_t* q, int have, uint2 b) {
+  if (WIDE) {
+    if (have > 0) *reinterpret_cast<uint2*>(q) = b;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+      if (j < have) q[j] = (uint8_t)((j < 4 ? b.x : b.y) >> (8 * (j & 3)));
+  }
+}
+
+__device__ __forceinline__ uint32_t largest_bits(const float (&v)[8]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) most = max_u32(most, __float_as_uint(v[j]) & 0x7fffffffu);
+  return most;
+}
+
+// Sixteen lanes hold one block, eight columns each. The block's largest
+// magnitude is compared as bits: a NaN is above infinity is above all numbers.
+// WIDE: rows and columns allow 16-byte loads and 8-byte stores (cols a multiple
+// of 8, so a lane's columns exist all or not at all).
+template <typename T, bool WIDE>
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(const T* __restrict__ x, size_t items,
+                                                           int cols, size_t ld,
+                                                           uint8_t* __restrict__ q,
+                                                           float* __restrict__ scales, int* err) {
+  const int nb = (cols + kFp8Block - 1) / kFp8Block;
+  const size_t item = ((size_t)blockIdx.x * 256 + threadIdx.x) / 16;
+  if (item >= items) return;
+  const size_t row = item / nb;
+  const int b = (int)(item % nb);
+  const int c = b * kFp8Block + (threadIdx.x & 15) * 8;
+  float v[8];
+  load8<T, WIDE>(x + row * ld + c, cols - c, v);
+  uint32_t most = largest_bits(v);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) most = max_u32(most, (uint32_t)__shfl_xor((int)most, o));
+  const uint32_t e = scale_exponent(most);
+  store8<WIDE>(q + row * cols + c, cols - c, to_fp8x8(v, __uint_as_float((254u - e) << 23)));
+  if ((threadIdx.x & 15) == 0) {
+    scales[item] = __uint_as_float(e << 23);
+    if (most >= 0x7f800000u) raise_error(err, kErrNumerical);
+  }
+}
+
+void launch_fp8_quantize(const void* x, int type, size_t rows, int cols, size_t ld, uint8_t* q,
+                         float* scales, int* err, hipStream_t s) {
+  const size_t nb = ((size_t)cols + kFp8Block - 1) / kFp8Block;
+  const size_t items = rows * nb;
+  const size_t size = type == kTypeF32 ? 4 : 2;
+  const bool wide = cols % 8 == 0 && (rows == 1 || ld * size % 16 == 0) &&
+                    reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+                    reinterpret_cast<uintptr_t>(q) % 8 == 0;
+  const dim3 grid((unsigned)((items + 15) / 16)), block(256);
+  if (type == kTypeF32) {
+    if (wide)
+      fp8_quantize_kernel<float, true><<<grid, block, 0, s>>>((const float*)x, items, cols, ld, q, scales, err);
+    else
+      fp8_quantize_kernel<float, false><<<grid, block, 0, s>>>((const float*)x, items, cols, ld, q, scales, err);
+  } else {
+    if (wide)
+      fp8_quantize_kernel<uint16_t, true><<<grid, block, 0, s>>>((const uint16_t*)x, items, cols, ld, q, scales, err);
+    else
+      fp8_quantize_kernel<uint16_t, false><<<grid, block, 0, s>>>((const uint16_t*)x, items, cols, ld, q, scales, err);
+  }
+}
+
+// One workgroup per 128 x 128 tile of a matrix (laid out once, not in a
+// serving path): sixteen lanes per row of the tile, sixteen rows per pass.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_quantize_tiles_kernel(const T* __restrict__ x, int rows,
+                                                                 int cols, size_t ld,
+                                                                 uint8_t* __restrict__ q,
+                                                                 float* __restrict__ scales,
+                                                                 int* err) {
+  __shared__ uint32_t wave_most[4];
+  const int c = (int)blockIdx.x * kFp8Block + (threadIdx.x & 15) * 8;
+  const int r0 = (int)blockIdx.y * kFp8Block + (threadIdx.x >> 4);
+  float v[8][8];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int r = r0 + 16 * i;
+    load8<T, false>(x + (size_t)r * ld + c, r < rows ? cols - c : 0, v[i]);
+    most = max_u32(most, largest_bits(v[i]));
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) most = max_u32(most, (uint32_t)__shfl_xor((int)most, o));
+  if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = max_u32(max_u32(wave_most[0], wave_most[1]), max_u32(wave_most[2], wave_most[3]));
+  const uint32_t e = scale_exponent(most);
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int r = r0 + 16 * i;
+    store8<false>(q + (size_t)r * cols + c, r < rows ? cols - c : 0,
+                  to_fp8x8(v[i], __uint_as_float((254u - e) << 23)));
+  }
+  if (threadIdx.x == 0) {
+    scales[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = __uint_as_float(e << 23);
+    if (most >= 0x7f800000u) raise_error(err, kErrNumerical);
+  }
+}
+
+void launch_fp8_quantize_tiles(const void* x, int type, int rows, int cols, size_t ld, uint8_t* q,
+                               float* scales, int* err, hipStream_t s) {
+  const dim3 grid((unsigned)((cols + kFp8Block - 1) / kFp8Block),
+                  (unsigned)((rows + kFp8Block - 1) / kFp8Block));
+  if (type == kTypeF32)
+    fp8_quantize_tiles_kernel<float><<<grid, 256, 0, s>>>((const float*)x, rows, cols, ld, q, scales, err);
+  else
+    fp8_quantize_tiles_kernel<uint16_t><<<grid, 256, 0, s>>>((const uint16_t*)x, rows, cols, ld, q, scales, err);
+}
+
+// ------------------------------------------------------------------ product
+
+// What a product leaves: its values in f32 or bf16, or its rows' statistics.
+enum { kOutF32, kOutBf16, kOutScores };
+
+struct ProductOut {
+  void* y;              // [m, n]
+  ScorePart* parts;     // [column tiles][m]
+  const int32_t* tokens;
+  float* given;         // [m] logits of the given tokens
+};
+
+// Sixteen bytes of a row of K bytes from byte k, zeros behind the row's end.
+// Rows start at any address where K is not a multiple of 16.
+__device__ __forceinline__ uint4 load_chunk(const uint8_t* row, int k, int K) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (k + 16 <= K) {
+    __builtin_memcpy(&v, row + k, 16);
+  } else {
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+      if (k + j < K) w[j / 4] |= (uint32_t)row[k + j] << (8 * (j & 3));
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+
+// Eight e4m3 values (two words) as bf16, which holds them exactly.
+__device__ __forceinline__ bf16x8 widen_fp8x8(uint32_t lo, uint32_t hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// 128 x 128 outputs per workgroup of four waves, 64 x 64 each. The matrix cores'
+// e4m3 instructions bring each group of eight products to the largest one's
+// exponent and cut them off 13 bits below it (measured: 2^16 - 2^16 + v keeps
+// multiples of 8; 1.3e-5 of a Gaussian block's sum), so the operands are widened
+// to bf16, whose products are summed to f32's last bit (1e-8). One scale block is
+// a chain of four v_mfma_f32_16x16x32_bf16 from zero, scaled into the f32
+// accumulators when it is done. The matrix is the first operand: lane l then
+// holds four adjacent columns of y for row l % 16, whose x scale it needs as one
+// value.
+template <int OUT>
+__global__ __launch_bounds__(256) void fp8_tile_kernel(Fp8Product p, ProductOut out) {
+  constexpr int kT = 128;
+  __shared__ __attribute__((aligned(16))) uint8_t lds_w[kT * 128], lds_x[kT * 128];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n0 = (int)blockIdx.x * kT, m0 = (int)blockIdx.y * kT;
+  const int wn = n0 + 64 * (wave & 1), wm = m0 + 64 * (wave >> 1);
+  const int fr = lane & 15, fg = lane >> 4;
+  const int K = p.k, nkb = p.kblocks();
+  f32x4 acc[4][4];  // [16 columns][16 rows]
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+
+  // Byte k of row r lies at chunk (k / 16) ^ (r % 8) of the row's 128 bytes:
+  // the sixteen rows of a fragment read then spread over all banks.
+  for (int kb = 0; kb < nkb; kb++) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int chunk = tid + 256 * i, r = chunk >> 3, c = chunk & 7;
+      const int at = r * 128 + 16 * (c ^ (r & 7));
+      uint4 a = make_uint4(0, 0, 0, 0), b = a;
+      if (n0 + r < p.n) a = load_chunk(p.w + (size_t)(n0 + r) * K, kb * 128 + 16 * c, K);
+      if (m0 + r < p.m) b = load_chunk(p.x + (size_t)(m0 + r) * K, kb * 128 + 16 * c, K);
+      *reinterpret_cast<uint4*>(lds_w + at) = a;
+      *reinterpret_cast<uint4*>(lds_x + at) = b;
+    }
+    __syncthreads();
+    const float ws = p.ws[(size_t)(n0 / kFp8Block) * nkb + kb];
+    // Lane group g takes chunks g and g + 4 of both operands: the order of
+    // the 128 products inside a block is free.
+    struct Fragment {
+      bf16x8 part[4];
+    };
+    auto fragment = [&](const uint8_t* tile, int r) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(tile + r * 128 + 16 * (fg ^ (r & 7)));
+      const uint4 hi = *reinterpret_cast<const uint4*>(tile + r * 128 + 16 * ((fg + 4) ^ (r & 7)));
+      return Fragment{{widen_fp8x8(lo.x, lo.y), widen_fp8x8(lo.z, lo.w), widen_fp8x8(hi.x, hi.y),
+                       widen_fp8x8(hi.z, hi.w)}};
+    };
+    Fragment fw[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) fw[i] = fragment(lds_w, wn - n0 + 16 * i + fr);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const Fragment fx = fragment(lds_x, wm - m0 + 16 * j + fr);
+      const int row = wm + 16 * j + fr;
+      const float sc = row < p.m ? p.xs[(size_t)row * nkb + kb] * ws : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 4; h++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i].part[h], fx.part[h], d, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[i][j][r] = fmaf(d[r], sc, acc[i][j][r]);
+      }
+    }
+  }
+
+  if constexpr (OUT == kOutScores) {
+    if (wn >= p.n) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int row = wm + 16 * j + fr;
+      const int token = out.tokens && row < p.m ? out.tokens[row] : -1;
+      ScorePart q = empty_part();
+      float most = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int col = wn + 16 * i + 4 * fg + r;
+          if (col >= p.n) continue;
+          most = fmaxf(most, acc[i][j][r]);
+          if (col == token) out.given[row] = acc[i][j][r];
+        }
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      q.r = most;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          if (wn + 16 * i + 4 * fg + r >= p.n) continue;
+          const float d = (acc[i][j][r] - q.r) * kLog2e;
+          const float e = __builtin_amdgcn_exp2f(d);
+          q.s += e;
+          q.t = fmaf(e, d, q.t);
+        }
+#pragma unroll
+      for (int o = 16; o <= 32; o <<= 1) {
+        q.s += __shfl_xor(q.s, o);
+        q.t += __shfl_xor(q.t, o);
+      }
+      if (fg == 0 && row < p.m) out.parts[(size_t)(wn / 64) * p.m + row] = q;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int row = wm + 16 * j + fr;
+      if (row >= p.m) continue;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int col = wn + 16 * i + 4 * fg + r;
+          if (col >= p.n) continue;
+          const size_t at = (size_t)row * p.n + col;
+          if (OUT == kOutF32)
+            static_cast<float*>(out.y)[at] = acc[i][j][r];
+          else
+            static_cast<uint16_t*>(out.y)[at] = bf16_bits(acc[i][j][r]);
+        }
+    }
+  }
+}
+
+static dim3 tile_grid(const Fp8Product& p) {
+  return dim3((unsigned)((p.n + 127) / 128), (unsigned)((p.m + 127) / 128));
+}
+
+void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, hipStream_t s) {
+  const ProductOut out{y, nullptr, nullptr, nullptr};
+  if (ytype == kTypeF32)
+    fp8_tile_kernel<kOutF32><<<tile_grid(p), 256, 0, s>>>(p, out);
+  else
+    fp8_tile_kernel<kOutBf16><<<tile_grid(p), 256, 0, s>>>(p, out);
+}
+
+// ------------------------------------------------- scores from the product
+
+static int score_tiles(const Fp8Product& p) { return (p.n + 63) / 64; }
+
+size_t fp8_score_bytes(const Fp8Product& p) {
+  return (size_t)score_tiles(p) * p.m * sizeof(ScorePart) + (size_t)p.m * 4;
+}
+
+// Joins the column tiles' statistics of each row. A workgroup takes `rows`
+// rows (a power of two, 1 to 64), 256 / rows threads each: adjacent threads
+// read adjacent rows of one tile.
+__global__ __launch_bounds__(256) void join_parts_kernel(const ScorePart* __restrict__ parts,
+                                                         int tiles, int m, int vocab, int rows,
+                                                         const float* __restrict__ given,
+                                                         TokenScores out, int* err) {
+  __shared__ ScorePart held[256];
+  const int tid = threadIdx.x;
+  const int row = (int)blockIdx.x * rows + (tid & (rows - 1));
+  ScorePart p = empty_part();
+  if (row < m)
+    for (int t = tid / rows; t < tiles; t += 256 / rows) p = join(p, parts[(size_t)t * m + row]);
+  held[tid] = p;
+  for (int o = 128; o >= rows; o >>= 1) {
+    __syncthreads();
+    if (tid < o) held[tid] = p = join(p, held[tid + o]);
+  }
+  if (tid >= rows || row >= m) return;
+  const int token = out.tokens ? out.tokens[row] : 0;
+  if (token < 0) {  // a padding row
+    if (out.logprobs) out.logprobs[row] = 0.0f;
+    if (out.entropy) out.entropy[row] = 0.0f;
+    return;
+  }
+  write_scores(out, row, token, vocab, p, out.logprobs && token < vocab ? given[row] : 0.0f, err);
+}
+
+void launch_fp8_scores(const Fp8Product& p, const TokenScores& out, void* work, int* err,
+                       hipStream_t s) {
+  const int tiles = score_tiles(p);
+  auto* parts = static_cast<ScorePart*>(work);
+  auto* given = reinterpret_cast<float*>(parts + (size_t)tiles * p.m);
+  const ProductOut po{nullptr, parts, out.logprobs ? out.tokens : nullptr, given};
+  fp8_tile_kernel<kOutScores><<<tile_grid(p), 256, 0, s>>>(p, po);
+  int rows = 1;
+  while (rows < 64 && rows * 2 <= p.m) rows *= 2;
+  join_parts_kernel<<<(unsigned)((p.m + rows - 1) / rows), 256, 0, s>>>(parts, tiles, p.m, p.n, rows,
+                                                                        given, out, err);
+}
+
+}  // namespace uocr

@@ -315,12 +315,12 @@ void launch_rms_norm(const float* x, int rows, int width, const RowNorm& nn, int
 // lmhead.hip: the vocabulary projection of one hidden row.
 struct LmHeadView {
   int V = 0, H = 0;
-  int kind = 0;                 // 0 BF16, 1 INT8 weight-only, 2 W8A8
+  int kind = 0;                 // 0 BF16, 1 INT8 weight-only, 2 W8A8, 3 FP8 blocks
   float eps = 0.0f;
   const float* norm_w = nullptr;  // [H] f32
   const uint16_t* w = nullptr;    // [V, H] bf16
-  const int8_t* q = nullptr;      // [V, H]
-  const float* s = nullptr;       // [V, H/32]
+  const int8_t* q = nullptr;      // [V, H] int8, or e4m3 bytes
+  const float* s = nullptr;       // [V, H/32]; FP8: [ceil(V/128), ceil(H/128)]
 };
 // The one-launch path: widths that are multiples of 64, up to 2048.
 bool lm_head_fast(int H);

@@ -26,7 +26,7 @@ LIB_PATH = os.environ.get("UOCR_MOE_LIB") or os.path.join(_HERE, "libuocr_moe.so
 
 OK, IO, JSON, FORMAT, SHAPE, UNSUPPORTED, RESOURCE, NUMERICAL = range(8)
 STATUS_NAMES = ["Ok", "Io", "Json", "Format", "Shape", "Unsupported", "Resource", "Numerical"]
-QUANT_NONE, QUANT_WEIGHTS_ONLY, QUANT_DYNAMIC = 0, 1, 2
+QUANT_NONE, QUANT_WEIGHTS_ONLY, QUANT_DYNAMIC, QUANT_FP8_BLOCKS = 0, 1, 2, 3
 MEMORY_HOST, MEMORY_DEVICE = 0, 1
 FLAG_FP32_CLASS = 0
 FLAG_BF16_ACTIVATIONS = 1
@@ -53,6 +53,10 @@ EXPORTS = [
     "uocr_lm_head_create", "uocr_lm_head_logits", "uocr_lm_head_logits_async",
     "uocr_lm_head_precision", "uocr_lm_head_device_bytes", "uocr_lm_head_destroy",
     "uocr_model_logits",
+    "uocr_fp8_quantize", "uocr_fp8_quantize_async", "uocr_fp8_quantize_weight",
+    "uocr_fp8_linear", "uocr_fp8_linear_async", "uocr_token_logprobs",
+    "uocr_token_logprobs_async", "uocr_fp8_linear_logprobs", "uocr_fp8_linear_logprobs_async",
+    "uocr_lm_head_logprobs", "uocr_lm_head_logprobs_async",
 ]
 DTYPES = ["BF16", "F16", "F32", "I64", "I8"]
 
@@ -211,6 +215,37 @@ def _load():
 
 
 lib = _load()
+
+
+class TokenScores(ctypes.Structure):
+    _fields_ = [("tokens", _P), ("n_top", _SZ), ("logprobs", _P), ("entropy", _P),
+                ("top_ids", _P), ("top_logprobs", _P)]
+
+
+# The 8-bit floating point operators and token scores. Bound at their first
+# call: a library built from the host sources alone does not have them.
+_QUANTIZE = [_P, _P, ctypes.c_int, _SZ, _SZ, _SZ, _P, _P]
+_PRODUCT = [_P, _P, _P, _SZ, _SZ, _P, _P, _SZ]
+_SCORES = ctypes.POINTER(TokenScores)
+_LATE = {
+    "uocr_fp8_quantize": _QUANTIZE,
+    "uocr_fp8_quantize_weight": _QUANTIZE,
+    "uocr_fp8_linear": _PRODUCT + [_P, ctypes.c_int],
+    "uocr_token_logprobs": [_P, _P, ctypes.c_int, _SZ, _SZ, _SZ, _SCORES],
+    "uocr_fp8_linear_logprobs": _PRODUCT + [_SCORES],
+    "uocr_lm_head_logprobs": [_P, _P, _P, _SZ, _SCORES],
+}
+_bound = {}
+
+
+def _operator(name: str, sync: bool = True):
+    fn = _bound.get((name, sync))
+    if fn is None:
+        fn = getattr(lib, name if sync else name + "_async")
+        fn.restype = ctypes.c_int
+        fn.argtypes = _LATE[name]
+        _bound[name, sync] = fn
+    return fn
 
 
 def _check(status: int):
@@ -376,7 +411,8 @@ class LmHead:
     """Decoder::logits: the last hidden row, RMSNorm with the final norm
     weight (f32 [H]), then the vocabulary projection — BF16 weight bits
     [V, H], or an INT8 overlay (q [V, H], scales [V, H/32]) weight-only or,
-    with QUANT_DYNAMIC_ACTIVATIONS, W8A8."""
+    with QUANT_DYNAMIC, W8A8; or, with QUANT_FP8_BLOCKS, e4m3 q [V, H] and
+    scales [ceil(V/128), ceil(H/128)]."""
 
     def __init__(self, ctx: Context, norm_weight, eps: float, weight=None, q=None, scales=None,
                  mode: int = 0, where: int = 0):
@@ -394,6 +430,14 @@ class LmHead:
     def logits(self, ctx: Context, hidden, out, sync: bool = True):
         fn = lib.uocr_lm_head_logits if sync else lib.uocr_lm_head_logits_async
         _check(fn(ctx.handle, self.handle, _ptr(hidden), hidden.shape[0], _ptr(out)))
+
+    def logprobs(self, ctx: Context, hidden, tokens=None, logprobs=None, entropy=None,
+                 top_ids=None, top_logprobs=None, sync: bool = True):
+        """Scores of the token after each row of hidden [T, H] (token_logprobs'
+        arguments)."""
+        s = _token_scores(hidden.shape[0], tokens, logprobs, entropy, top_ids, top_logprobs)
+        _check(_operator("uocr_lm_head_logprobs", sync)(ctx.handle, self.handle, _ptr(hidden),
+                                                        hidden.shape[0], ctypes.byref(s)))
 
     @property
     def precision(self) -> str:
@@ -457,6 +501,116 @@ def int8_linear_dynamic(ctx: Context, q, scales, x, y, block_sums=None):
 def rms_norm(ctx: Context, x, weight, eps: float, out):
     rows, width = x.shape
     _check(lib.uocr_rms_norm(ctx.handle, _ptr(x), rows, width, _ptr(weight), eps, _ptr(out)))
+
+
+# ---------------------------------------- 8-bit floating point, token scores
+
+FP8_BLOCK = 128
+MAX_TOP = 64
+
+
+def _shape(ok: bool, message: str):
+    if not ok:
+        raise UocrError(SHAPE, message)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // FP8_BLOCK)
+
+
+_TYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}
+
+
+def _type(t) -> int:
+    """uocr_dtype of a floating torch tensor (others: Unsupported)."""
+    code = _TYPES.get(str(t.dtype))
+    if code is None:
+        raise UocrError(UNSUPPORTED, f"element type {t.dtype}")
+    return code
+
+
+def _rows(t, what: str) -> int:
+    """The row stride of a 2-D tensor whose rows are contiguous."""
+    _shape(t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), f"{what} must be rows")
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _quantize(name, ctx, x, q, scales, scale_rows, sync):
+    ld = _rows(x, "x")
+    rows, cols = x.shape
+    _shape(tuple(q.shape) == (rows, cols) and q.is_contiguous() and q.element_size() == 1,
+           "q must be contiguous bytes of x's shape")
+    _shape(tuple(scales.shape) == (scale_rows, _blocks(cols)) and scales.is_contiguous(),
+           "scales must be one per block")
+    _check(_operator(name, sync)(ctx.handle, x.data_ptr(), _type(x), rows, cols, ld,
+                                 q.data_ptr(), scales.data_ptr()))
+
+
+def fp8_quantize(ctx: Context, x, q, scales, sync: bool = True):
+    """Rows x [rows, cols] (f32 or bf16, any row stride) to e4m3 q [rows, cols]
+    (float8_e4m3fn or uint8) and f32 scales [rows, ceil(cols / 128)]."""
+    _quantize("uocr_fp8_quantize", ctx, x, q, scales, x.shape[0], sync)
+
+
+def fp8_quantize_weight(ctx: Context, w, q, scales):
+    """A matrix w [rows, cols] to e4m3 with scales [ceil(rows / 128),
+    ceil(cols / 128)], one per 128 x 128 tile."""
+    _quantize("uocr_fp8_quantize_weight", ctx, w, q, scales, _blocks(w.shape[0]), True)
+
+
+def _product(xq, xs, wq, ws):
+    """The product's arguments (uocr_fp8_linear's second to eighth)."""
+    _shape(xq.dim() == 2 and wq.dim() == 2 and xq.shape[1] == wq.shape[1],
+           "x [m, k] and w [n, k] must agree")
+    m, k = xq.shape
+    n = wq.shape[0]
+    _shape(tuple(xs.shape) == (m, _blocks(k)) and tuple(ws.shape) == (_blocks(n), _blocks(k)),
+           "scales must be [m, blocks(k)] and [blocks(n), blocks(k)]")
+    _shape(xq.is_contiguous() and wq.is_contiguous() and xs.is_contiguous() and ws.is_contiguous()
+           and xq.element_size() == 1 and wq.element_size() == 1 and xs.element_size() == 4
+           and ws.element_size() == 4, "product operands must be contiguous e4m3 and f32")
+    return xq.data_ptr(), xs.data_ptr(), m, k, wq.data_ptr(), ws.data_ptr(), n
+
+
+def fp8_linear(ctx: Context, xq, xs, wq, ws, y, sync: bool = True):
+    """y [m, n] (f32 or bf16) = x . w^T of e4m3 rows xq [m, k] with scales xs and
+    an e4m3 matrix wq [n, k] with scales ws per 128 x 128 tile."""
+    args = _product(xq, xs, wq, ws)
+    _shape(tuple(y.shape) == (args[2], args[6]) and y.is_contiguous(), "y must be [m, n]")
+    _check(_operator("uocr_fp8_linear", sync)(ctx.handle, *args, y.data_ptr(), _type(y)))
+
+
+def _token_scores(rows, tokens, logprobs, entropy, top_ids, top_logprobs) -> TokenScores:
+    n_top = top_ids.shape[1] if top_ids is not None else 0
+    for t, shape, size in ((tokens, (rows,), 4), (logprobs, (rows,), 4), (entropy, (rows,), 4),
+                           (top_ids, (rows, n_top), 4), (top_logprobs, (rows, n_top), 4)):
+        _shape(t is None or (tuple(t.shape) == shape and t.is_contiguous()
+                             and t.element_size() == size),
+               "score arrays must be contiguous 32-bit values, one per row (and alternative)")
+    return TokenScores(_ptr(tokens), n_top, _ptr(logprobs), _ptr(entropy), _ptr(top_ids),
+                       _ptr(top_logprobs))
+
+
+def token_logprobs(ctx: Context, logits, tokens=None, logprobs=None, entropy=None, top_ids=None,
+                   top_logprobs=None, sync: bool = True):
+    """Scores of logits [rows, vocab] (f32, bf16 or f16, any row stride): the log
+    probability of tokens [rows] (int32; negative: a padding row), the entropy,
+    and the most probable ids top_ids [rows, n] (int32) with their log
+    probabilities. Outputs are f32 tensors to fill; None skips one."""
+    ld = _rows(logits, "logits")
+    rows, vocab = logits.shape
+    s = _token_scores(rows, tokens, logprobs, entropy, top_ids, top_logprobs)
+    _check(_operator("uocr_token_logprobs", sync)(ctx.handle, logits.data_ptr(), _type(logits),
+                                                  rows, vocab, ld, ctypes.byref(s)))
+
+
+def fp8_linear_logprobs(ctx: Context, xq, xs, wq, ws, tokens=None, logprobs=None, entropy=None,
+                        top_ids=None, top_logprobs=None, sync: bool = True):
+    """token_logprobs of fp8_linear's product, without its logits in memory
+    unless alternatives are asked for."""
+    args = _product(xq, xs, wq, ws)
+    s = _token_scores(args[2], tokens, logprobs, entropy, top_ids, top_logprobs)
+    _check(_operator("uocr_fp8_linear_logprobs", sync)(ctx.handle, *args, ctypes.byref(s)))
 
 
 # --------------------------------------------------------------- files
