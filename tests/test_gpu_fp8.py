@@ -278,6 +278,43 @@ def test_linear_random(ctx, m, n, k):
     assert (off <= tol + 2.0 ** -8 * (np.abs(want) + tol)).all()
 
 
+def device_exact(m, n, k, seed):
+    """exact_product made on the device, with its result there in float64."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    codes = {int(v): i for i, v in enumerate(E4M3) if v == v and v == int(v) and abs(v) <= 4}
+    lut = torch.tensor([codes[v] for v in range(-4, 5)], dtype=torch.uint8, device="cuda")
+
+    def operand(rows, tile):
+        v = torch.randint(0, 9, (rows, k), generator=g, device="cuda")
+        s = 2.0 ** torch.randint(0, 4, (blocks(rows) if tile else rows, blocks(k)), generator=g, device="cuda")
+        f = s.repeat_interleave(128, 1)[:, :k]
+        f = f.repeat_interleave(128, 0)[:rows] if tile else f
+        return lut[v], s.float(), (v - 4).double() * f
+    x, xs, a = operand(m, False)
+    w, ws, b = operand(n, True)
+    return (x, xs, w, ws), torch.mm(a, b.t().contiguous())
+
+
+# Vocabularies: whole and ragged columns and depths, x small and too large for LDS.
+@pytest.mark.parametrize("m,n,k", [(1, 65536, 1280), (1, 129280, 1280), (3, 70001, 272), (16, 65549, 128),
+                                   (17, 66000, 144), (33, 129280, 640), (48, 65600, 1280), (64, 65537, 1296),
+                                   (64, 65700, 2400), (1, 66000, 6848), (5, 65530, 16)])
+def test_linear_wide_exact(ctx, m, n, k):
+    say(f"wide product {m}x{n}x{k}")
+    ops, want = device_exact(m, n, k, m + n)
+    guard = torch.full((m * n + 64,), 12345.0, device="cuda")
+    y = guard[:m * n].view(m, n)
+    torch.cuda.synchronize()
+    um.fp8_linear(ctx, *ops, y)
+    assert torch.equal(y.double(), want)
+    assert bool((guard[m * n:] == 12345.0).all())
+    y16 = torch.empty((m, n), device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    um.fp8_linear(ctx, *ops, y16)
+    assert torch.equal(y16, want.float().to(torch.bfloat16))
+
+
 @pytest.mark.parametrize("m", [1, 20, 150, 300])
 def test_linear_nan_bytes_stay_in_their_row_and_column(ctx, m):
     n, k = 300, 400

@@ -18,7 +18,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import uocr_moe as um  # noqa: E402
-from test_gpu_fp8 import blocks, device_product, exact_product, random_product, say, spread  # noqa: E402
+from test_gpu_fp8 import blocks, device_exact, device_product, exact_product, random_product, say, spread  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -312,6 +312,21 @@ def test_linear_logprobs_random(ctx, m, n, k):
     compare(out.host(), reference(a @ b.T, tokens, 0), extra)
     um.fp8_linear_logprobs(ctx, *dev, t, **again.views())
     assert all(np.array_equal(out.host()[x], again.host()[x]) for x in out.host())
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 129280, 1280), (2, 65536, 144), (19, 70001, 256), (48, 66003, 640),
+                                   (64, 65700, 2400)])
+def test_linear_logprobs_wide(ctx, m, n, k):
+    say(f"wide fused scores {m}x{n}x{k}")
+    (x, xs, w, ws), logits = device_exact(m, n, k, m + n)
+    factor = 2.0 ** -round(math.log2(64 * math.sqrt(k)))
+    tokens = np.random.default_rng(m).integers(0, n, m).astype(np.int32)
+    tokens[-1] = n - 1
+    want = reference((logits * factor).cpu().numpy(), tokens, 0)
+    out, t, xs = Scores(m, 0), torch.from_numpy(tokens).cuda(), xs * factor
+    torch.cuda.synchronize()
+    um.fp8_linear_logprobs(ctx, x, xs, w, ws, t, **out.views())
+    compare(out.host(), want)
 
 
 @pytest.mark.parametrize("m", [3, 200])

@@ -709,6 +709,7 @@ int uocr_gpu_ctx_create(int device, size_t scratch_limit, uocr_gpu_ctx** out) {
   std::call_once(g_attr_once, [] {
     uocr::gemv_init_attributes();
     uocr::mfma_init_attributes();
+    uocr::fp8_init_attributes();
   });
   auto* ctx = new uocr_gpu_ctx();
   ctx->device = device;
@@ -1091,6 +1092,7 @@ int uocr_moe_forward_static(const uocr_moe_layer* layer, const float* x, size_t 
   std::call_once(g_attr_once, [] {
     uocr::gemv_init_attributes();
     uocr::mfma_init_attributes();
+    uocr::fp8_init_attributes();
   });
   char* base = nullptr;
   if (int r = static_scratch_of(layer->device, &base)) return r;

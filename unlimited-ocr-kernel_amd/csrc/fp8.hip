@@ -5,6 +5,8 @@
 //
 // No counterpart in the reference, whose overlay is int8 with blocks of 32
 // (src/cpu/quantized.rs:9-237); these stand beside its operators.
+#include <algorithm>
+
 #include "fp8.hpp"
 #include "mfma.hpp"
 #include "scores.hpp"
@@ -227,6 +229,67 @@ __device__ __forceinline__ bf16x8 widen_fp8x8(uint32_t lo, uint32_t hi) {
   return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Four adjacent columns of row `row`, from column col on.
+template <int OUT>
+__device__ __forceinline__ void store_columns(const Fp8Product& p, void* y, int row, int col, f32x4 v) {
+  if (row >= p.m || col >= p.n) return;
+  const size_t at = (size_t)row * p.n + col;
+  if (p.n % 4 == 0) {  // four whole columns; y is aligned to its element, so is any of its rows to four
+    if (OUT == kOutF32) {
+      __builtin_memcpy(static_cast<float*>(y) + at, &v, 16);
+    } else {
+      const uint2 b = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+      __builtin_memcpy(static_cast<uint16_t*>(y) + at, &b, 8);
+    }
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    if (col + r >= p.n) return;
+    if (OUT == kOutF32)
+      static_cast<float*>(y)[at + r] = v[r];
+    else
+      static_cast<uint16_t*>(y)[at + r] = bf16_bits(v[r]);
+  }
+}
+
+// The statistics of one row's logits in a wave: lane l holds columns col + 16 i +
+// r of row l % 16 (v[i][r]; col differs between the four lanes of a row). Every
+// lane of the row gets them. The lane with the given token's column keeps its logit.
+template <int COUNT>
+__device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int col, int n, int token,
+                                                    float* given) {
+  ScorePart q = empty_part();
+  float most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < COUNT; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int c = col + 16 * i + r;
+      if (c >= n) continue;
+      most = fmaxf(most, v[i][r]);
+      if (c == token) *given = v[i][r];
+    }
+  most = fmaxf(most, __shfl_xor(most, 16));
+  q.r = fmaxf(most, __shfl_xor(most, 32));
+#pragma unroll
+  for (int i = 0; i < COUNT; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      if (col + 16 * i + r >= n) continue;
+      const float d = (v[i][r] - q.r) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(d);
+      q.s += e;
+      q.t = fmaf(e, d, q.t);
+    }
+#pragma unroll
+  for (int o = 16; o <= 32; o <<= 1) {
+    q.s += __shfl_xor(q.s, o);
+    q.t += __shfl_xor(q.t, o);
+  }
+  return q;
+}
+
 // 128 x 128 outputs per workgroup of four waves, 64 x 64 each. The matrix cores'
 // e4m3 instructions bring each group of eight products to the largest one's
 // exponent and cut them off 13 bits below it (measured: 2^16 - 2^16 + v keeps
@@ -303,55 +366,15 @@ __global__ __launch_bounds__(256) void fp8_tile_kernel(Fp8Product p, ProductOut 
     for (int j = 0; j < 4; j++) {
       const int row = wm + 16 * j + fr;
       const int token = out.tokens && row < p.m ? out.tokens[row] : -1;
-      ScorePart q = empty_part();
-      float most = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int col = wn + 16 * i + 4 * fg + r;
-          if (col >= p.n) continue;
-          most = fmaxf(most, acc[i][j][r]);
-          if (col == token) out.given[row] = acc[i][j][r];
-        }
-      most = fmaxf(most, __shfl_xor(most, 16));
-      most = fmaxf(most, __shfl_xor(most, 32));
-      q.r = most;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          if (wn + 16 * i + 4 * fg + r >= p.n) continue;
-          const float d = (acc[i][j][r] - q.r) * kLog2e;
-          const float e = __builtin_amdgcn_exp2f(d);
-          q.s += e;
-          q.t = fmaf(e, d, q.t);
-        }
-#pragma unroll
-      for (int o = 16; o <= 32; o <<= 1) {
-        q.s += __shfl_xor(q.s, o);
-        q.t += __shfl_xor(q.t, o);
-      }
+      const f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+      const ScorePart q = row_statistics<4>(v, wn + 4 * fg, p.n, token, out.given + row);
       if (fg == 0 && row < p.m) out.parts[(size_t)(wn / 64) * p.m + row] = q;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int row = wm + 16 * j + fr;
-      if (row >= p.m) continue;
+    for (int j = 0; j < 4; j++)
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const int col = wn + 16 * i + 4 * fg + r;
-          if (col >= p.n) continue;
-          const size_t at = (size_t)row * p.n + col;
-          if (OUT == kOutF32)
-            static_cast<float*>(out.y)[at] = acc[i][j][r];
-          else
-            static_cast<uint16_t*>(out.y)[at] = bf16_bits(acc[i][j][r]);
-        }
-    }
+      for (int i = 0; i < 4; i++) store_columns<OUT>(p, out.y, wm + 16 * j + fr, wn + 16 * i + 4 * fg, acc[i][j]);
   }
 }
 
@@ -359,20 +382,432 @@ static dim3 tile_grid(const Fp8Product& p) {
   return dim3((unsigned)((p.n + 127) / 128), (unsigned)((p.m + 127) / 128));
 }
 
-void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, hipStream_t s) {
-  const ProductOut out{y, nullptr, nullptr, nullptr};
-  if (ytype == kTypeF32)
-    fp8_tile_kernel<kOutF32><<<tile_grid(p), 256, 0, s>>>(p, out);
+// ---- few rows (at most 64): the matrix is streamed from memory straight to the
+// registers of the wave that multiplies it, two scale blocks in flight; x comes
+// from the caches. A wave takes 16 RG columns of y (rows of the matrix) and all of
+// x's rows, as MB blocks of 16; KS waves of a workgroup share a group's depth and
+// add up in LDS, in order. Lane l reads the bytes [16 (l / 16), +16) and 64 bytes
+// on of row l % 16 in each block: a load instruction covers 64-byte runs.
+constexpr int kStreamRows = 64;
+constexpr int kCus = 256, kMostLds = 160 << 10;
+
+struct StreamShape {
+  int ks, waves;  // waves that share a group's depth, waves per workgroup
+};
+
+// Most waves of a workgroup, by the registers that a wave then may have: 128 where
+// x has one or two blocks of rows and a wave one group of columns, 256 otherwise.
+constexpr int stream_waves(int mb, int rg) { return rg == 1 ? (mb <= 2 ? 16 : 8) : 4; }
+
+template <int MB, int RG, int OUT>
+__global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kernel(Fp8Product p, ProductOut out, StreamShape shape) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fg = lane >> 4;
+  const int groups = shape.waves / shape.ks;  // of this workgroup
+  const int slot = wave / shape.ks, k0 = wave % shape.ks;
+  const int n0 = ((int)blockIdx.x * groups + slot) * 16 * RG;
+  const int K = p.k, nkb = p.kblocks();
+
+  struct Stage {
+    uint4 w[RG][2], x[MB][2];
+    float xs[MB], ws;
+  };
+  f32x4 acc[RG][MB];
+#pragma unroll
+  for (int i = 0; i < RG; i++)
+#pragma unroll
+    for (int j = 0; j < MB; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+
+  if (n0 < p.n) {
+    // Rows past the last one read the last one's bytes; what comes of them is not
+    // stored. Bytes past a row's end are zeros on both sides.
+    const uint8_t* wrow[RG];
+#pragma unroll
+    for (int i = 0; i < RG; i++) wrow[i] = p.w + (size_t)min(n0 + 16 * i + fr, p.n - 1) * K + 16 * fg;
+    const uint8_t* xrow[MB];
+    const float* xsrow[MB];
+#pragma unroll
+    for (int j = 0; j < MB; j++) {
+      const int row = min(16 * j + fr, p.m - 1);
+      xrow[j] = p.x + (size_t)row * K + 16 * fg;
+      xsrow[j] = p.xs + (size_t)row * nkb;
+    }
+    const float* wsrow = p.ws + (size_t)(n0 / kFp8Block) * nkb;
+    auto load = [&](Stage& s, int kb) {
+      const int k = kb * kFp8Block;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const bool in = k + 64 * h + 16 * fg < K;  // K is a multiple of 16
+#pragma unroll
+        for (int i = 0; i < RG; i++)
+          s.w[i][h] = in ? *reinterpret_cast<const uint4*>(wrow[i] + k + 64 * h) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < MB; j++)
+          s.x[j][h] = in ? *reinterpret_cast<const uint4*>(xrow[j] + k + 64 * h) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < MB; j++) s.xs[j] = xsrow[j][kb];
+      s.ws = wsrow[kb];
+    };
+    auto multiply = [&](const Stage& s) {
+      bf16x8 fw[RG][4];
+#pragma unroll
+      for (int i = 0; i < RG; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          fw[i][2 * h] = widen_fp8x8(s.w[i][h].x, s.w[i][h].y);
+          fw[i][2 * h + 1] = widen_fp8x8(s.w[i][h].z, s.w[i][h].w);
+        }
+#pragma unroll
+      for (int j = 0; j < MB; j++) {
+        const float sc = s.xs[j] * s.ws;
+        bf16x8 fx[4];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          fx[2 * h] = widen_fp8x8(s.x[j][h].x, s.x[j][h].y);
+          fx[2 * h + 1] = widen_fp8x8(s.x[j][h].z, s.x[j][h].w);
+        }
+#pragma unroll
+        for (int i = 0; i < RG; i++) {
+          f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int h = 0; h < 4; h++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i][h], fx[h], d, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; r++) acc[i][j][r] = fmaf(d[r], sc, acc[i][j][r]);
+        }
+      }
+    };
+    Stage a, b;
+    int kb = k0;
+    if (kb < nkb) load(a, kb);
+    while (kb < nkb) {
+      if (kb + shape.ks < nkb) load(b, kb + shape.ks);
+      multiply(a);
+      kb += shape.ks;
+      if (kb >= nkb) break;
+      if (kb + shape.ks < nkb) load(a, kb + shape.ks);
+      multiply(b);
+      kb += shape.ks;
+    }
+  }
+
+  // The waves of a group add up into its first one.
+  if (shape.ks > 1) {
+    f32x4* held = reinterpret_cast<f32x4*>(lds);
+    if (k0 > 0)
+#pragma unroll
+      for (int i = 0; i < RG; i++)
+#pragma unroll
+        for (int j = 0; j < MB; j++) held[(wave * RG * MB + i * MB + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    if (k0 == 0)
+      for (int w = 1; w < shape.ks; w++)
+#pragma unroll
+        for (int i = 0; i < RG; i++)
+#pragma unroll
+          for (int j = 0; j < MB; j++) {
+            const f32x4 o = held[((wave + w) * RG * MB + i * MB + j) * 64 + lane];
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[i][j][r] += o[r];
+          }
+  }
+  if constexpr (OUT == kOutScores) {
+    // One part per workgroup and row: the groups' join in LDS.
+    ScorePart* held = reinterpret_cast<ScorePart*>(lds);
+    if (shape.ks > 1) __syncthreads();
+    if (k0 == 0)
+#pragma unroll
+      for (int j = 0; j < MB; j++) {
+        const int row = 16 * j + fr;
+        const int token = out.tokens && row < p.m ? out.tokens[row] : -1;
+        f32x4 v[RG];
+#pragma unroll
+        for (int i = 0; i < RG; i++) v[i] = acc[i][j];
+        const ScorePart q = row_statistics<RG>(v, n0 + 4 * fg, p.n, token, out.given + row);
+        if (fg == 0) held[slot * (16 * MB) + row] = n0 < p.n ? q : empty_part();
+      }
+    __syncthreads();
+    if (tid < 16 * MB && tid < p.m) {
+      ScorePart q = held[tid];
+      for (int g = 1; g < groups; g++) q = join(q, held[g * (16 * MB) + tid]);
+      out.parts[(size_t)blockIdx.x * p.m + tid] = q;
+    }
+  } else {
+    if (k0 == 0)
+#pragma unroll
+      for (int j = 0; j < MB; j++)
+#pragma unroll
+        for (int i = 0; i < RG; i++) store_columns<OUT>(p, out.y, 16 * j + fr, n0 + 16 * i + 4 * fg, acc[i][j]);
+  }
+}
+
+// Whole 16-byte chunks of rows at aligned addresses.
+static bool whole_chunks(const Fp8Product& p) {
+  return p.k % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0;
+}
+
+static bool takes_stream(const Fp8Product& p) { return p.m <= kStreamRows && whole_chunks(p); }
+
+// The depth is split until there are some 2048 waves.
+struct StreamPlan {
+  int rg, mb;
+  StreamShape shape;
+  int grid;
+  size_t lds;
+};
+static StreamPlan plan_stream(const Fp8Product& p, bool scores) {
+  StreamPlan s;
+  s.mb = (p.m + 15) / 16;
+  s.rg = (p.n + 31) / 32 >= 2048 ? 2 : 1;
+  const int groups = (p.n + 16 * s.rg - 1) / (16 * s.rg);
+  int ks = 1;
+  while (ks < stream_waves(s.mb, s.rg) && groups * ks < 2048 && ks * 2 <= p.kblocks()) ks *= 2;
+  s.shape.ks = ks;
+  s.shape.waves = ks < 4 ? 4 : ks;
+  const int per = s.shape.waves / ks;
+  s.grid = (groups + per - 1) / per;
+  s.lds = ks > 1 ? (size_t)s.shape.waves * s.rg * s.mb * 64 * sizeof(f32x4) : 0;
+  if (scores) s.lds = std::max(s.lds, (size_t)per * 16 * s.mb * sizeof(ScorePart));
+  return s;
+}
+
+template <int MB, int RG>
+static void run_stream(const Fp8Product& p, const ProductOut& out, int kind, const StreamPlan& t, hipStream_t s) {
+  const dim3 grid(t.grid), block(64 * t.shape.waves);
+  if (kind == kOutF32)
+    fp8_stream_kernel<MB, RG, kOutF32><<<grid, block, t.lds, s>>>(p, out, t.shape);
+  else if (kind == kOutBf16)
+    fp8_stream_kernel<MB, RG, kOutBf16><<<grid, block, t.lds, s>>>(p, out, t.shape);
   else
+    fp8_stream_kernel<MB, RG, kOutScores><<<grid, block, t.lds, s>>>(p, out, t.shape);
+}
+template <int RG>
+static void run_stream_rows(const Fp8Product& p, const ProductOut& out, int kind, const StreamPlan& t, hipStream_t s) {
+  if (t.mb == 1) run_stream<1, RG>(p, out, kind, t, s);
+  if (t.mb == 2) run_stream<2, RG>(p, out, kind, t, s);
+  if (t.mb == 3) run_stream<3, RG>(p, out, kind, t, s);
+  if (t.mb == 4) run_stream<4, RG>(p, out, kind, t, s);
+}
+
+// ---- few rows and many columns (a vocabulary): persistent workgroups of eight
+// waves, one per CU, hold x in LDS and stream the matrix with kWideDepth scale
+// blocks of 32 columns in flight per wave, across the ends of groups. Scores stay
+// in registers until the last group: one part per workgroup and row.
+constexpr int kWideWaves = 8, kWideDepth = 4, kWideCols = 32;
+
+struct WideShape {
+  int groups;  // of kWideCols columns
+};
+
+constexpr size_t kWideParts = (size_t)kWideWaves * kStreamRows * sizeof(ScorePart);
+static size_t wide_lds(const Fp8Product& p) {
+  const size_t rows = (size_t)(p.m + 15) / 16 * 16;
+  return rows * p.kblocks() * (kFp8Block + sizeof(float)) + kWideParts;
+}
+
+template <int MB, int OUT>
+__global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product p, ProductOut out, WideShape shape) {
+  constexpr int D = kWideDepth, R = kWideCols / 16;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fg = lane >> 4;
+  const int K = p.k, nkb = p.kblocks();
+  char* xl = lds;                                                        // [kb][16 MB rows][128]
+  float* xsl = reinterpret_cast<float*>(lds + (size_t)nkb * MB * 16 * kFp8Block);  // [kb][16 MB rows]
+  ScorePart* held = reinterpret_cast<ScorePart*>(xsl + nkb * MB * 16);
+
+  struct Stage {
+    uint4 w[R][2];
+    float ws;
+  };
+  auto load = [&](Stage& s, int g, int kb) {
+    const int n0 = g * kWideCols, k = kb * kFp8Block + 16 * fg;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      const uint8_t* row = p.w + (size_t)min(n0 + 16 * i + fr, p.n - 1) * K + k;
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        s.w[i][h] = k + 64 * h < K ? *reinterpret_cast<const uint4*>(row + 64 * h) : make_uint4(0, 0, 0, 0);
+    }
+    s.ws = p.ws[(size_t)(n0 / kFp8Block) * nkb + kb];
+  };
+  const int stride = (int)gridDim.x * kWideWaves;
+  int g = (int)blockIdx.x * kWideWaves + wave;
+  Stage ring[D];
+#pragma unroll
+  for (int d = 0; d < D; d++)
+    if (g < shape.groups && d < nkb) load(ring[d], g, d);
+
+  // x: chunk c of a row's 128 bytes at c ^ (row % 8), so that the sixteen rows of
+  // a fragment read spread over all banks; zeros behind the last row and column.
+  for (int c = tid; c < nkb * MB * 16 * 8; c += 64 * kWideWaves) {
+    const int kb = c / (MB * 16 * 8), row = c / 8 % (MB * 16), k = kb * kFp8Block + 16 * (c & 7);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < p.m && k < K) v = *reinterpret_cast<const uint4*>(p.x + (size_t)row * K + k);
+    *reinterpret_cast<uint4*>(xl + ((size_t)kb * MB * 16 + row) * 128 + 16 * ((c & 7) ^ (row & 7))) = v;
+  }
+  for (int c = tid; c < nkb * MB * 16; c += 64 * kWideWaves) {
+    const int kb = c / (MB * 16), row = c % (MB * 16);
+    xsl[c] = row < p.m ? p.xs[(size_t)row * nkb + kb] : 0.0f;
+  }
+  __syncthreads();
+
+  ScorePart sum[MB];
+  int token[MB];
+  if constexpr (OUT == kOutScores)
+#pragma unroll
+    for (int j = 0; j < MB; j++) {
+      sum[j] = empty_part();
+      token[j] = out.tokens && 16 * j + fr < p.m ? out.tokens[16 * j + fr] : -1;
+    }
+  for (; g < shape.groups; g += stride) {
+    f32x4 acc[R][MB];
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int j = 0; j < MB; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = 0; k0 < nkb; k0 += D) {
+#pragma unroll
+      for (int d = 0; d < D; d++) {
+        const int kb = k0 + d;
+        if (kb < nkb) {
+          const Stage& s = ring[d];
+          bf16x8 fw[R][4];
+#pragma unroll
+          for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              fw[i][2 * h] = widen_fp8x8(s.w[i][h].x, s.w[i][h].y);
+              fw[i][2 * h + 1] = widen_fp8x8(s.w[i][h].z, s.w[i][h].w);
+            }
+          const char* xb = xl + (size_t)kb * MB * 16 * 128;
+#pragma unroll
+          for (int j = 0; j < MB; j++) {
+            const int row = 16 * j + fr;
+            bf16x8 fx[4];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+              const uint4 v = *reinterpret_cast<const uint4*>(xb + row * 128 + 16 * ((fg + 4 * h) ^ (row & 7)));
+              fx[2 * h] = widen_fp8x8(v.x, v.y);
+              fx[2 * h + 1] = widen_fp8x8(v.z, v.w);
+            }
+            const float sc = xsl[kb * MB * 16 + row] * s.ws;
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+              f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+              for (int h = 0; h < 4; h++) v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i][h], fx[h], v, 0, 0, 0);
+#pragma unroll
+              for (int r = 0; r < 4; r++) acc[i][j][r] = fmaf(v[r], sc, acc[i][j][r]);
+            }
+          }
+        }
+        // The slot's next block: of this group, or behind its last blocks the next
+        // group's block d.
+        if (kb + D < nkb)
+          load(ring[d], g, kb + D);
+        else if (k0 + D >= nkb && d < nkb && g + stride < shape.groups)
+          load(ring[d], g + stride, d);
+      }
+    }
+    const int n0 = g * kWideCols;
+#pragma unroll
+    for (int j = 0; j < MB; j++) {
+      if constexpr (OUT == kOutScores) {
+        f32x4 v[R];
+#pragma unroll
+        for (int i = 0; i < R; i++) v[i] = acc[i][j];
+        sum[j] = join(sum[j], row_statistics<R>(v, n0 + 4 * fg, p.n, token[j], out.given + 16 * j + fr));
+      } else {
+#pragma unroll
+        for (int i = 0; i < R; i++) store_columns<OUT>(p, out.y, 16 * j + fr, n0 + 16 * i + 4 * fg, acc[i][j]);
+      }
+    }
+  }
+  if constexpr (OUT == kOutScores) {
+#pragma unroll
+    for (int j = 0; j < MB; j++)
+      if (fg == 0) held[wave * (16 * MB) + 16 * j + fr] = sum[j];
+    __syncthreads();
+    if (tid < 16 * MB && tid < p.m) {
+      ScorePart q = held[tid];
+      for (int w = 1; w < kWideWaves; w++) q = join(q, held[w * (16 * MB) + tid]);
+      out.parts[(size_t)blockIdx.x * p.m + tid] = q;
+    }
+  }
+}
+
+template <int MB>
+static void run_wide(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s) {
+  const dim3 grid(kCus), block(64 * kWideWaves);
+  const WideShape shape{(p.n + kWideCols - 1) / kWideCols};
+  const size_t lds = wide_lds(p);
+  if (kind == kOutF32)
+    fp8_wide_kernel<MB, kOutF32><<<grid, block, lds, s>>>(p, out, shape);
+  else if (kind == kOutBf16)
+    fp8_wide_kernel<MB, kOutBf16><<<grid, block, lds, s>>>(p, out, shape);
+  else
+    fp8_wide_kernel<MB, kOutScores><<<grid, block, lds, s>>>(p, out, shape);
+}
+
+template <int MB>
+static void wide_attributes() {
+  const void* kernels[] = {(const void*)fp8_wide_kernel<MB, kOutF32>, (const void*)fp8_wide_kernel<MB, kOutBf16>,
+                           (const void*)fp8_wide_kernel<MB, kOutScores>};
+  for (const void* k : kernels) (void)hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
+}
+void fp8_init_attributes() {
+  wide_attributes<1>();
+  wide_attributes<2>();
+  wide_attributes<3>();
+  wide_attributes<4>();
+  (void)hipGetLastError();  // a refused attribute surfaces at launch instead
+}
+
+// Enough columns to keep every wave at work, and x fits into LDS.
+static bool takes_wide(const Fp8Product& p) {
+  return p.n >= kCus * kWideWaves * kWideCols && wide_lds(p) <= (size_t)kMostLds;
+}
+
+static void launch_product(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s) {
+  if (takes_stream(p) && takes_wide(p)) {
+    const int mb = (p.m + 15) / 16;
+    if (mb == 1) run_wide<1>(p, out, kind, s);
+    if (mb == 2) run_wide<2>(p, out, kind, s);
+    if (mb == 3) run_wide<3>(p, out, kind, s);
+    if (mb == 4) run_wide<4>(p, out, kind, s);
+  } else if (takes_stream(p)) {
+    const StreamPlan t = plan_stream(p, kind == kOutScores);
+    t.rg == 2 ? run_stream_rows<2>(p, out, kind, t, s) : run_stream_rows<1>(p, out, kind, t, s);
+  } else if (kind == kOutF32) {
+    fp8_tile_kernel<kOutF32><<<tile_grid(p), 256, 0, s>>>(p, out);
+  } else if (kind == kOutBf16) {
     fp8_tile_kernel<kOutBf16><<<tile_grid(p), 256, 0, s>>>(p, out);
+  } else {
+    fp8_tile_kernel<kOutScores><<<tile_grid(p), 256, 0, s>>>(p, out);
+  }
+}
+
+void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, hipStream_t s) {
+  launch_product(p, {y, nullptr, nullptr, nullptr}, ytype == kTypeF32 ? kOutF32 : kOutBf16, s);
 }
 
 // ------------------------------------------------- scores from the product
 
-static int score_tiles(const Fp8Product& p) { return (p.n + 63) / 64; }
+// Parts per row.
+static int score_tiles(const Fp8Product& p) {
+  if (!takes_stream(p)) return (p.n + 63) / 64;
+  return takes_wide(p) ? kCus : plan_stream(p, true).grid;
+}
 
 size_t fp8_score_bytes(const Fp8Product& p) {
-  return (size_t)score_tiles(p) * p.m * sizeof(ScorePart) + (size_t)p.m * 4;
+  // Room for p.m rows or fewer, whichever kernel takes them.
+  const size_t few = std::min(p.m, kStreamRows);
+  return std::max((size_t)((p.n + 63) / 64) * p.m, (size_t)((p.n + 15) / 16) * few) * sizeof(ScorePart) +
+         (size_t)p.m * 4;
 }
 
 // Joins the column tiles' statistics of each row. A workgroup takes `rows`
@@ -409,7 +844,7 @@ void launch_fp8_scores(const Fp8Product& p, const TokenScores& out, void* work, 
   auto* parts = static_cast<ScorePart*>(work);
   auto* given = reinterpret_cast<float*>(parts + (size_t)tiles * p.m);
   const ProductOut po{nullptr, parts, out.logprobs ? out.tokens : nullptr, given};
-  fp8_tile_kernel<kOutScores><<<tile_grid(p), 256, 0, s>>>(p, po);
+  launch_product(p, po, kOutScores, s);
   int rows = 1;
   while (rows < 64 && rows * 2 <= p.m) rows *= 2;
   join_parts_kernel<<<(unsigned)((p.m + rows - 1) / rows), 256, 0, s>>>(parts, tiles, p.m, p.n, rows,

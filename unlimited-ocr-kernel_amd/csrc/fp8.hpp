@@ -20,6 +20,9 @@ void launch_fp8_quantize(const void* x, int type, size_t rows, int cols, size_t 
 void launch_fp8_quantize_tiles(const void* x, int type, int rows, int cols, size_t ld, uint8_t* q,
                                float* scales, int* err, hipStream_t s);
 
+// Once per process, before the first launch.
+void fp8_init_attributes();
+
 // One product: x [m, k] e4m3 rows with scales [m, blocks(k)], w [n, k] with
 // scales [blocks(n), blocks(k)].
 struct Fp8Product {
