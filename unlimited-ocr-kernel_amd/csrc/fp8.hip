@@ -810,32 +810,49 @@ size_t fp8_score_bytes(const Fp8Product& p) {
          (size_t)p.m * 4;
 }
 
-// Joins the column tiles' statistics of each row. A workgroup takes `rows`
-// rows (a power of two, 1 to 64), 256 / rows threads each: adjacent threads
-// read adjacent rows of one tile.
-__global__ __launch_bounds__(256) void join_parts_kernel(const ScorePart* __restrict__ parts,
-                                                         int tiles, int m, int vocab, int rows,
-                                                         const float* __restrict__ given,
-                                                         TokenScores out, int* err) {
-  __shared__ ScorePart held[256];
-  const int tid = threadIdx.x;
-  const int row = (int)blockIdx.x * rows + (tid & (rows - 1));
+// Joins the column tiles' statistics of each row. A workgroup of sixteen waves
+// takes R rows (1, 4, 16 or 64, the wave's lanes being R rows of 64 / R tiles each,
+// so that adjacent lanes read adjacent rows' parts): every thread some tiles, four
+// loads in flight, then the lanes and the waves of a row. With one row or some
+// dozens each thread has about one part: two dependent reads of memory in all.
+constexpr int kJoinWaves = 16;
+
+template <int R>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_parts_kernel(const ScorePart* __restrict__ parts,
+                                                                     int tiles, int m, int vocab,
+                                                                     const float* __restrict__ given,
+                                                                     TokenScores out, int* err) {
+  __shared__ ScorePart held[kJoinWaves][R];
+  constexpr int kStep = 64 * kJoinWaves / R;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane % R, row = (int)blockIdx.x * R + r;
+  const int token = row < m && out.tokens ? out.tokens[row] : 0;
+  const float logit = row < m && out.logprobs && token >= 0 && token < vocab ? given[row] : 0.0f;
   ScorePart p = empty_part();
-  if (row < m)
-    for (int t = tid / rows; t < tiles; t += 256 / rows) p = join(p, parts[(size_t)t * m + row]);
-  held[tid] = p;
-  for (int o = 128; o >= rows; o >>= 1) {
-    __syncthreads();
-    if (tid < o) held[tid] = p = join(p, held[tid + o]);
+  if (row < m) {
+    const ScorePart* at = parts + row;
+    for (int t = threadIdx.x / R; t < tiles; t += 4 * kStep) {
+      ScorePart q[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        q[i] = empty_part();
+        if (t + i * kStep < tiles) q[i] = at[(size_t)(t + i * kStep) * m];
+      }
+      p = join(p, join(join(q[0], q[1]), join(q[2], q[3])));
+    }
   }
-  if (tid >= rows || row >= m) return;
-  const int token = out.tokens ? out.tokens[row] : 0;
+#pragma unroll
+  for (int o = 32; o >= R; o >>= 1) p = join(p, shfl_xor(p, o));
+  if (lane < R) held[wave][lane] = p;
+  __syncthreads();
+  if (wave > 0 || lane >= R || row >= m) return;
   if (token < 0) {  // a padding row
     if (out.logprobs) out.logprobs[row] = 0.0f;
     if (out.entropy) out.entropy[row] = 0.0f;
     return;
   }
-  write_scores(out, row, token, vocab, p, out.logprobs && token < vocab ? given[row] : 0.0f, err);
+  for (int w = 1; w < kJoinWaves; w++) p = join(p, held[w][r]);
+  write_scores(out, row, token, vocab, p, logit, err);
 }
 
 void launch_fp8_scores(const Fp8Product& p, const TokenScores& out, void* work, int* err,
@@ -845,10 +862,18 @@ void launch_fp8_scores(const Fp8Product& p, const TokenScores& out, void* work, 
   auto* given = reinterpret_cast<float*>(parts + (size_t)tiles * p.m);
   const ProductOut po{nullptr, parts, out.logprobs ? out.tokens : nullptr, given};
   launch_product(p, po, kOutScores, s);
-  int rows = 1;
-  while (rows < 64 && rows * 2 <= p.m) rows *= 2;
-  join_parts_kernel<<<(unsigned)((p.m + rows - 1) / rows), 256, 0, s>>>(parts, tiles, p.m, p.n, rows,
-                                                                        given, out, err);
+#define UOCR_JOIN(R)                                                                               \
+  join_parts_kernel<R><<<(unsigned)((p.m + R - 1) / R), 64 * kJoinWaves, 0, s>>>(parts, tiles, p.m, p.n, \
+                                                                                 given, out, err)
+  if (p.m < 4)
+    UOCR_JOIN(1);
+  else if (p.m < 64)
+    UOCR_JOIN(4);
+  else if (p.m < 1024)
+    UOCR_JOIN(16);
+  else
+    UOCR_JOIN(64);
+#undef UOCR_JOIN
 }
 
 }  // namespace uocr

@@ -1,14 +1,14 @@
 // Scores of logits in memory: the log probability of each row's given token,
 // the entropy of its distribution, and its most probable tokens.
 //
-// One pass over the logits (scores.hpp has the mathematics) leaves, per chunk
-// of a row, its statistics and, where alternatives are asked for, the largest
-// logit of every group of adjacent columns. The n largest logits of a row lie
-// in the n groups with the largest maxima (of equal ones, the leftmost): each
-// group in front of another holds an element that comes before all of the
-// other's. So the second launch, one workgroup per row, joins the statistics,
-// picks n groups from the maxima (1/64 or 1/128 of the row) and reads only
-// those again.
+// One pass over the logits (scores.hpp has the mathematics) leaves, per wave's
+// chunk of a row, its statistics and, where alternatives are asked for, the largest
+// logit of every group of 16 lanes' columns (64 or 128). The second launch, one
+// workgroup per row, joins the statistics and finds the alternatives from the
+// maxima without ordering them: with tau the n-th largest of its threads' maxima, at
+// least n logits are not below tau, so the n largest logits are among the logits
+// that are not below tau in the groups whose maximum is not. Those are few unless
+// many are equal; each is ranked by counting the ones before it.
 #include <algorithm>
 
 #include "fp8.hpp"
@@ -42,31 +42,28 @@ struct Logits<_Float16> {
 static int vec_of(int type) { return type == kTypeF32 ? 4 : 8; }
 static int group_of(int type) { return 16 * vec_of(type); }
 
-// Vectors per thread of a chunk: large chunks where there are many rows, small
-// ones where a few rows have to fill the card.
-static int chunk_vectors(size_t rows, int vocab, int type) {
-  int v = 8;
-  while (v > 1 && rows * (((size_t)vocab + kScoreThreads * vec_of(type) * v - 1) /
-                          (kScoreThreads * vec_of(type) * v)) < 2048)
-    v /= 2;
-  return v;
+// Vectors per lane of a wave's chunk, all in flight at once: eight where there are
+// many rows, fewer where a few rows have to fill the card (some 2048 waves).
+constexpr int kMostVectors = 8;
+static size_t chunks_of(int vocab, int type, int vectors) {
+  const size_t chunk = (size_t)64 * vec_of(type) * vectors;
+  return ((size_t)vocab + chunk - 1) / chunk;
 }
 
 struct ScorePlan {
-  int vectors, chunk, chunks, groups;
+  int vectors, chunks, groups;
   size_t maxima_at, bytes;
 };
 static ScorePlan plan_scores(size_t rows, int vocab, int type, int top) {
   ScorePlan p;
-  p.vectors = chunk_vectors(rows, vocab, type);
-  p.chunk = kScoreThreads * vec_of(type) * p.vectors;
-  p.chunks = (int)(((size_t)vocab + p.chunk - 1) / p.chunk);
+  p.vectors = kMostVectors;
+  while (p.vectors > 1 && rows * chunks_of(vocab, type, p.vectors) < 2048) p.vectors /= 2;
+  p.chunks = (int)chunks_of(vocab, type, p.vectors);
   p.groups = (int)(((size_t)vocab + group_of(type) - 1) / group_of(type));
   // Room for `rows` rows or fewer: fewer rows may take smaller chunks (at most
-  // 2 * 2047 of them in all, or one vector per thread each).
-  const size_t unit = (size_t)kScoreThreads * vec_of(type);
-  const size_t most = std::max(rows * (((size_t)vocab + 8 * unit - 1) / (8 * unit)),
-                               std::min<size_t>(4096, rows * (((size_t)vocab + unit - 1) / unit)));
+  // 2 * 2047 of them in all, or one vector per lane each).
+  const size_t most = std::max(rows * chunks_of(vocab, type, kMostVectors),
+                               std::min<size_t>(4096, rows * chunks_of(vocab, type, 1)));
   p.maxima_at = most * sizeof(ScorePart);
   p.bytes = p.maxima_at + (top ? rows * p.groups * sizeof(float) : 0);
   return p;
@@ -77,11 +74,9 @@ size_t token_score_bytes(size_t rows, int vocab, int type, int top) {
 }
 
 size_t token_score_rows(int vocab, int type) {
-  // Many rows take chunks of eight vectors per thread.
-  const size_t chunk = (size_t)kScoreThreads * vec_of(type) * 8;
-  const size_t chunks = ((size_t)vocab + chunk - 1) / chunk;
-  const size_t rows = (((size_t)1 << 24) - 1) / chunks;
-  return rows < ((size_t)1 << 22) ? (rows ? rows : 1) : (size_t)1 << 22;
+  const size_t chunks = chunks_of(vocab, type, kMostVectors);
+  const size_t rows = (((size_t)1 << 26) - 1) / chunks;  // 64 threads each
+  return std::min(std::max<size_t>(rows, 1), (size_t)1 << 22);
 }
 
 // One vector of a row as f32, -inf behind the row's end. Rows may start at any
@@ -100,52 +95,64 @@ __device__ __forceinline__ void load_logits(const T* row, int c, int vocab, floa
   }
 }
 
-template <typename T>
+// Largest of the sixteen lanes of a row of lanes, in each of them.
+__device__ __forceinline__ float row16_max(float v) {
+  v = fmaxf(v, dpp_move<0xB1>(v));   // quad_perm [1,0,3,2]
+  v = fmaxf(v, dpp_move<0x4E>(v));   // quad_perm [2,3,0,1]
+  v = fmaxf(v, dpp_move<0x141>(v));  // row_half_mirror
+  v = fmaxf(v, dpp_move<0x140>(v));  // row_mirror
+  return v;
+}
+
+template <typename T, int V>
 __global__ __launch_bounds__(kScoreThreads) void score_chunks_kernel(
-    const T* __restrict__ logits, int vocab, size_t ld, const int32_t* __restrict__ tokens,
-    int vectors, int chunks, ScorePart* __restrict__ parts, float* __restrict__ maxima, int groups) {
+    const T* __restrict__ logits, size_t items, int vocab, size_t ld, const int32_t* __restrict__ tokens,
+    int chunks, ScorePart* __restrict__ parts, float* __restrict__ maxima, int groups) {
   constexpr int kVec = Logits<T>::kVec;
-  __shared__ ScorePart held[kScoreThreads / 64];
-  const size_t row = blockIdx.x / (unsigned)chunks;
-  const int chunk = (int)(blockIdx.x % (unsigned)chunks);
+  const int lane = threadIdx.x & 63;
+  const size_t item = (size_t)blockIdx.x * (kScoreThreads / 64) +
+                      (size_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  if (item >= items) return;
+  const size_t row = item / (unsigned)chunks;
+  const int chunk = (int)(item % (unsigned)chunks);
   if (tokens && tokens[row] < 0) return;  // a padding row is not read
   const T* x = logits + row * ld;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  ScorePart p = empty_part();
-  for (int i = 0; i < vectors; i++) {
-    const int c = ((chunk * vectors + i) * kScoreThreads + tid) * kVec;
-    float v[kVec];
-    load_logits<T>(x, c, vocab, v);
-    float most = v[0];
+  const int c0 = (chunk * V * 64 + lane) * kVec;
+  float v[V][kVec];
 #pragma unroll
-    for (int j = 1; j < kVec; j++) most = fmaxf(most, v[j]);
-    ScorePart q = empty_part();
-    bool nan = false;
+  for (int i = 0; i < V; i++) load_logits<T>(x, c0 + i * 64 * kVec, vocab, v[i]);
+  float most = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kVec; j++) nan |= v[j] != v[j];
-    if (most > -INFINITY || nan) {
-      q.r = most;
+  for (int i = 0; i < V; i++) {
+    float g = v[i][0];
 #pragma unroll
-      for (int j = 0; j < kVec; j++) {
-        const float d = (v[j] - q.r) * kLog2e;
-        const float e = __builtin_amdgcn_exp2f(d);
-        q.s += e;
-        q.t = fmaf(e, fmaxf(d, -1000.0f), q.t);  // a banned word: 0 times -inf is 0 here
-      }
-    }
-    p = join(p, q);
-    if (maxima) {
-      float g = most;
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor(g, o));
-      if ((lane & 15) == 0 && c < vocab) maxima[row * groups + c / (16 * kVec)] = g;
-    }
+    for (int j = 1; j < kVec; j++) g = fmaxf(g, v[i][j]);
+    g = row16_max(g);
+    most = fmaxf(most, g);
+    const int c = c0 + i * 64 * kVec;
+    if (maxima && (lane & 15) == 0 && c < vocab) maxima[row * groups + c / (16 * kVec)] = g;
   }
+  most = fmaxf(most, __shfl_xor(most, 16));
+  most = fmaxf(most, __shfl_xor(most, 32));
+  ScorePart p = empty_part();
+  p.r = most;
+  // A chunk of banned words has no reference; with 0 in its place every term
+  // vanishes (and a NaN stays one).
+  const float r = most == -INFINITY ? 0.0f : most;
+  float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) p = join(p, shfl_xor(p, o));
-  if (lane == 0) held[wave] = p;
-  __syncthreads();
-  if (tid == 0) parts[blockIdx.x] = join(join(held[0], held[1]), join(held[2], held[3]));
+  for (int i = 0; i < V; i++)
+#pragma unroll
+    for (int j = 0; j < kVec; j++) {
+      // A banned word's distance is brought to where 2^d is 0 and 0 times d too.
+      const float d = (v[i][j] - r) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(d);
+      s[j & 1] += e;
+      t[j & 1] = fmaf(e, fmaxf(d, -1000.0f), t[j & 1]);
+    }
+  p.s = wave_sum(s[0] + s[1]);
+  p.t = wave_sum(t[0] + t[1]);
+  if (lane == 0) parts[item] = p;
 }
 
 // The workgroup's largest key.
@@ -161,15 +168,22 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long key,
   return best;
 }
 
+// Groups and candidates that the short way holds; more (many equal logits) take
+// the long one, which passes over the row once for each alternative.
+constexpr int kMostGroups = 512, kMostCandidates = 1024;
+
 template <typename T>
 __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     const T* __restrict__ logits, int vocab, size_t ld, int chunks,
     const ScorePart* __restrict__ parts, const float* __restrict__ maxima, int groups,
     TokenScores out, int* err) {
-  constexpr int kGroup = 16 * Logits<T>::kVec;
+  constexpr int kVec = Logits<T>::kVec, kGroup = 16 * kVec;
   __shared__ ScorePart held[kScoreThreads / 64];
-  __shared__ unsigned long long keys[kScoreThreads / 64];
-  __shared__ int picked[kMaxTop];
+  __shared__ unsigned long long keys[kMostCandidates];
+  __shared__ int listed[kMostGroups];
+  __shared__ float mine[kScoreThreads];
+  __shared__ float tau_at;
+  __shared__ int counts[2];
   const size_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int token = out.tokens ? out.tokens[row] : 0;
@@ -183,17 +197,31 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     }
     return;
   }
+  const T* x = logits + row * ld;
+  const float* gmax = maxima + row * groups;
+  const float given = tid == 0 && out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f;
   ScorePart p = empty_part();
   for (int c = tid; c < chunks; c += kScoreThreads) p = join(p, parts[row * chunks + c]);
+  // This thread's largest group.
+  float most = -INFINITY;
+  if (top)
+    for (int g = tid; g < groups; g += kScoreThreads) most = fmaxf(most, gmax[g]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) p = join(p, shfl_xor(p, o));
   if (lane == 0) held[wave] = p;
+  // Up to sixteen alternatives need 64 maxima to choose tau from: four lanes' each.
+  const int many = top <= 16 ? kScoreThreads / 4 : kScoreThreads;
+  if (top <= 16) {
+    most = fmaxf(most, dpp_move<0xB1>(most));
+    most = fmaxf(most, dpp_move<0x4E>(most));
+    if ((tid & 3) == 0) mine[tid >> 2] = most;
+  } else {
+    mine[tid] = most;
+  }
+  if (tid < 2) counts[tid] = 0;
   __syncthreads();
   p = join(join(held[0], held[1]), join(held[2], held[3]));
-  const T* x = logits + row * ld;
-  if (tid == 0)
-    write_scores(out, row, token, vocab, p,
-                 out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f, err);
+  if (tid == 0) write_scores(out, row, token, vocab, p, given, err);
   if (top == 0) return;
   if (!has_distribution(p)) {
     for (int i = tid; i < top; i += kScoreThreads) {
@@ -202,35 +230,69 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     }
     return;
   }
-  // The groups, in order; keys are distinct, so each is the largest below the
-  // one before it.
-  const int some = min(top, groups);
-  unsigned long long last = ~0ull;
-  for (int i = 0; i < some; i++) {
-    unsigned long long best = 0;
-    for (int g = tid; g < groups; g += kScoreThreads) {
-      const unsigned long long key = order_key(maxima[row * groups + g], (uint32_t)g);
-      if (key < last && key > best) best = key;
-    }
-    last = block_max(best, keys);
-    if (tid == 0) picked[i] = (int)key_index(last);
+  if (tid < many) {
+    const float v = mine[tid];
+    int before = 0;
+    for (int i = 0; i < many; i++) before += mine[i] > v || (mine[i] == v && i < tid);
+    if (before == top - 1) tau_at = v;
   }
   __syncthreads();
-  const float l = log2f(p.s);
-  last = ~0ull;
+  const float tau = tau_at;
+  // With tau -inf (fewer finite logits than alternatives, or nearly): all finite
+  // logits, and the first columns' banned ones to fill up with.
+  const bool finite = tau > -INFINITY;
+  for (int g = tid; g < groups; g += kScoreThreads)
+    if (finite ? gmax[g] >= tau : gmax[g] > -INFINITY || g == 0) {
+      const int at = atomicAdd(&counts[0], 1);
+      if (at < kMostGroups) listed[at] = g;
+    }
+  __syncthreads();
+  const int some = counts[0];
+  if (some <= kMostGroups) {
+    for (int i = tid; i < some * kGroup; i += kScoreThreads) {
+      const int col = listed[i / kGroup] * kGroup + i % kGroup;
+      if (col >= vocab) continue;
+      const float v = Logits<T>::widen(x[col]);
+      if (finite ? v >= tau : v > -INFINITY || col < top) {
+        const int at = atomicAdd(&counts[1], 1);
+        if (at < kMostCandidates) keys[at] = order_key(v, (uint32_t)col);
+      }
+    }
+    __syncthreads();
+  }
+  const float l = kLn2 * log2f(p.s);
+  auto write = [&](int at, unsigned long long key) {
+    out.top_ids[row * top + at] = (int32_t)key_index(key);
+    out.top_logprobs[row * top + at] = key_value(key) - p.r - l;
+  };
+  const int found = counts[1];
+  if (some <= kMostGroups && found <= kMostCandidates) {
+    // The order of the list differs from run to run; the ranks do not.
+    for (int i = tid; i < found; i += kScoreThreads) {
+      const unsigned long long key = keys[i];
+      int before = 0;
+      for (int j = 0; j < found; j++) before += keys[j] > key;
+      if (before < top) write(before, key);
+    }
+    return;
+  }
+  // The long way: one alternative after the other, each the largest below the one
+  // before it.
+  __syncthreads();
+  unsigned long long last = ~0ull;
   for (int i = 0; i < top; i++) {
     unsigned long long best = 0;
-    for (int c = tid; c < some * kGroup; c += kScoreThreads) {
-      const int col = picked[c / kGroup] * kGroup + c % kGroup;
-      if (col >= vocab) continue;
-      const unsigned long long key = order_key(Logits<T>::widen(x[col]), (uint32_t)col);
-      if (key < last && key > best) best = key;
+    for (int c = tid * kVec; c < vocab; c += kScoreThreads * kVec) {
+      float v[kVec];
+      load_logits<T>(x, c, vocab, v);
+#pragma unroll
+      for (int j = 0; j < kVec; j++) {
+        const unsigned long long key = order_key(v[j], (uint32_t)(c + j));
+        if (c + j < vocab && key < last && key > best) best = key;
+      }
     }
     last = block_max(best, keys);
-    if (tid == 0) {
-      out.top_ids[row * top + i] = (int32_t)key_index(last);
-      out.top_logprobs[row * top + i] = key_value(last) - p.r - kLn2 * l;
-    }
+    if (tid == 0) write(i, last);
   }
 }
 
@@ -239,8 +301,20 @@ static void launch(const T* logits, size_t rows, int vocab, size_t ld, const Sco
                    const TokenScores& out, void* work, int* err, hipStream_t s) {
   auto* parts = static_cast<ScorePart*>(work);
   float* maxima = out.top ? reinterpret_cast<float*>(static_cast<char*>(work) + plan.maxima_at) : nullptr;
-  score_chunks_kernel<T><<<(unsigned)(rows * plan.chunks), kScoreThreads, 0, s>>>(
-      logits, vocab, ld, out.tokens, plan.vectors, plan.chunks, parts, maxima, plan.groups);
+  const size_t items = rows * plan.chunks;
+  const dim3 grid((unsigned)((items + kScoreThreads / 64 - 1) / (kScoreThreads / 64))), block(kScoreThreads);
+#define UOCR_CHUNKS(V)                                                                             \
+  score_chunks_kernel<T, V><<<grid, block, 0, s>>>(logits, items, vocab, ld, out.tokens, plan.chunks, \
+                                                   parts, maxima, plan.groups)
+  if (plan.vectors == 8)
+    UOCR_CHUNKS(8);
+  else if (plan.vectors == 4)
+    UOCR_CHUNKS(4);
+  else if (plan.vectors == 2)
+    UOCR_CHUNKS(2);
+  else
+    UOCR_CHUNKS(1);
+#undef UOCR_CHUNKS
   score_rows_kernel<T><<<(unsigned)rows, kScoreThreads, 0, s>>>(logits, vocab, ld, plan.chunks, parts,
                                                                 maxima, plan.groups, out, err);
 }
