@@ -14,6 +14,12 @@
 namespace uocr {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A raw buffer resource for loads: those at or past `bytes` give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t read_rsrc(const void* base, uint32_t bytes) {
+  return store_rsrc(const_cast<void*>(base), bytes);
+}
 
 // ------------------------------------------------------------- quantisation
 
@@ -395,6 +401,8 @@ struct StreamShape {
   int ks, waves;  // waves that share a group's depth, waves per workgroup
 };
 
+// Blocks in flight.
+constexpr int kStreamDepth = 2;
 // Most waves of a workgroup, by the registers that a wave then may have: 128 where
 // x has one or two blocks of rows and a wave one group of columns, 256 otherwise.
 constexpr int stream_waves(int mb, int rg) { return rg == 1 ? (mb <= 2 ? 16 : 8) : 4; }
@@ -411,7 +419,7 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
   const int K = p.k, nkb = p.kblocks();
 
   struct Stage {
-    uint4 w[RG][2], x[MB][2];
+    u32x4 w[RG][2], x[MB][2];
     float xs[MB], ws;
   };
   f32x4 acc[RG][MB];
@@ -421,35 +429,30 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
     for (int j = 0; j < MB; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
   if (n0 < p.n) {
-    // Rows past the last one read the last one's bytes; what comes of them is not
-    // stored. Bytes past a row's end are zeros on both sides.
-    const uint8_t* wrow[RG];
-#pragma unroll
-    for (int i = 0; i < RG; i++) wrow[i] = p.w + (size_t)min(n0 + 16 * i + fr, p.n - 1) * K + 16 * fg;
-    const uint8_t* xrow[MB];
-    const float* xsrow[MB];
-#pragma unroll
-    for (int j = 0; j < MB; j++) {
-      const int row = min(16 * j + fr, p.m - 1);
-      xrow[j] = p.x + (size_t)row * K + 16 * fg;
-      xsrow[j] = p.xs + (size_t)row * nkb;
-    }
-    const float* wsrow = p.ws + (size_t)(n0 / kFp8Block) * nkb;
+    // Rows past the last one and chunks past a row's end are out of the resources'
+    // ranges: zeros, without a branch around the loads (as in the kernel below).
+    const __amdgpu_buffer_rsrc_t rw = read_rsrc(p.w + (size_t)n0 * K, (uint32_t)min(16 * RG, p.n - n0) * K);
+    const __amdgpu_buffer_rsrc_t rx = read_rsrc(p.x, (uint32_t)p.m * K);
+    const __amdgpu_buffer_rsrc_t rs = read_rsrc(p.xs, (uint32_t)(p.m * nkb) * 4u);
+    const __amdgpu_buffer_rsrc_t rt = read_rsrc(p.ws + (size_t)(n0 / kFp8Block) * nkb, (uint32_t)nkb * 4u);
     auto load = [&](Stage& s, int kb) {
-      const int k = kb * kFp8Block;
+      const int k = kb * kFp8Block + 16 * fg;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const bool in = k + 64 * h + 16 * fg < K;  // K is a multiple of 16
+        const int out_of = k + 64 * h < K ? 0 : (int)kDmaOut;  // K is a multiple of 16
 #pragma unroll
         for (int i = 0; i < RG; i++)
-          s.w[i][h] = in ? *reinterpret_cast<const uint4*>(wrow[i] + k + 64 * h) : make_uint4(0, 0, 0, 0);
+          s.w[i][h] = __builtin_amdgcn_raw_buffer_load_b128(rw, ((16 * i + fr) * K + k + 64 * h) | out_of, 0, 0);
 #pragma unroll
         for (int j = 0; j < MB; j++)
-          s.x[j][h] = in ? *reinterpret_cast<const uint4*>(xrow[j] + k + 64 * h) : make_uint4(0, 0, 0, 0);
+          s.x[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rx, ((16 * j + fr) * K + k + 64 * h) | out_of, 0, 0);
       }
+      const int past = kb < nkb ? 0 : (int)kDmaOut;
 #pragma unroll
-      for (int j = 0; j < MB; j++) s.xs[j] = xsrow[j][kb];
-      s.ws = wsrow[kb];
+      for (int j = 0; j < MB; j++)
+        s.xs[j] =
+            __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, ((16 * j + fr) * nkb + kb) * 4 | past, 0, 0));
+      s.ws = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rt, kb * 4 | past, 0, 0));
     };
     auto multiply = [&](const Stage& s) {
       bf16x8 fw[RG][4];
@@ -479,17 +482,16 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
         }
       }
     };
-    Stage a, b;
-    int kb = k0;
-    if (kb < nkb) load(a, kb);
-    while (kb < nkb) {
-      if (kb + shape.ks < nkb) load(b, kb + shape.ks);
-      multiply(a);
-      kb += shape.ks;
-      if (kb >= nkb) break;
-      if (kb + shape.ks < nkb) load(a, kb + shape.ks);
-      multiply(b);
-      kb += shape.ks;
+    constexpr int D = kStreamDepth;
+    Stage ring[D];
+#pragma unroll
+    for (int d = 0; d < D; d++) load(ring[d], k0 + d * shape.ks);
+    for (int kb = k0; kb < nkb; kb += D * shape.ks) {
+#pragma unroll
+      for (int d = 0; d < D; d++) {  // those past the last block multiply zeros
+        multiply(ring[d]);
+        load(ring[d], kb + (d + D) * shape.ks);
+      }
     }
   }
 
@@ -550,7 +552,6 @@ static bool whole_chunks(const Fp8Product& p) {
 
 static bool takes_stream(const Fp8Product& p) { return p.m <= kStreamRows && whole_chunks(p); }
 
-// The depth is split until there are some 2048 waves.
 struct StreamPlan {
   int rg, mb;
   StreamShape shape;
@@ -562,11 +563,15 @@ static StreamPlan plan_stream(const Fp8Product& p, bool scores) {
   s.mb = (p.m + 15) / 16;
   s.rg = (p.n + 31) / 32 >= 2048 ? 2 : 1;
   const int groups = (p.n + 16 * s.rg - 1) / (16 * s.rg);
-  int ks = 1;
-  while (ks < stream_waves(s.mb, s.rg) && groups * ks < 2048 && ks * 2 <= p.kblocks()) ks *= 2;
+  // Waves of a group: as many as fill the card, then as few as leave each the same
+  // whole rounds of kStreamDepth blocks.
+  const int want = std::min({stream_waves(s.mb, s.rg), p.kblocks(), (2048 + groups - 1) / groups});
+  int each = (p.kblocks() + want - 1) / want;
+  each = (each + kStreamDepth - 1) / kStreamDepth * kStreamDepth;
+  const int ks = (p.kblocks() + each - 1) / each;
+  const int per = std::max(1, 4 / ks);
   s.shape.ks = ks;
-  s.shape.waves = ks < 4 ? 4 : ks;
-  const int per = s.shape.waves / ks;
+  s.shape.waves = per * ks;
   s.grid = (groups + per - 1) / per;
   s.lds = ks > 1 ? (size_t)s.shape.waves * s.rg * s.mb * 64 * sizeof(f32x4) : 0;
   if (scores) s.lds = std::max(s.lds, (size_t)per * 16 * s.mb * sizeof(ScorePart));
@@ -595,7 +600,11 @@ static void run_stream_rows(const Fp8Product& p, const ProductOut& out, int kind
 // waves, one per CU, hold x in LDS and stream the matrix with kWideDepth scale
 // blocks of 32 columns in flight per wave, across the ends of groups. Scores stay
 // in registers until the last group: one part per workgroup and row.
-constexpr int kWideWaves = 8, kWideDepth = 4, kWideCols = 32;
+// 129280 x 1280 (165 MB): one row 34 us (4.8 TB/s; the same loads alone take 28.5),
+// 48 rows 37 us, 64 rows 42 us. Four or five blocks in flight are slower (35 and 40
+// us for one and 48 rows), as are two workgroups per CU, and waves that load x from
+// the caches instead (39 and 66 us).
+constexpr int kWideWaves = 8, kWideDepth = 2, kWideCols = 32;
 
 struct WideShape {
   int groups;  // of kWideCols columns
@@ -620,39 +629,79 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
   ScorePart* held = reinterpret_cast<ScorePart*>(xsl + nkb * MB * 16);
 
   struct Stage {
-    uint4 w[R][2];
+    u32x4 w[R][2];
     float ws;
   };
+  // Every load is issued whatever is left to do, without a branch: what lies past a
+  // row's last chunk, a group's last row or the wave's last group is out of its
+  // resource's range and comes as zeros. Around a branch the compiler waits for all
+  // loads instead of the oldest block's (37 -> 35 us for 129280 x 1280 and one row).
+  // The tile scales come by vector loads for the same reason: scalar ones return in
+  // no order, so each would be waited for with all others.
+  const int tiles = (p.n + kFp8Block - 1) / kFp8Block;
+  const __amdgpu_buffer_rsrc_t rt = read_rsrc(p.ws, (uint32_t)(tiles * nkb) * 4u);
   auto load = [&](Stage& s, int g, int kb) {
     const int n0 = g * kWideCols, k = kb * kFp8Block + 16 * fg;
+    const int rows = g < shape.groups ? min(kWideCols, p.n - n0) : 0;
+    const __amdgpu_buffer_rsrc_t rs = read_rsrc(p.w + (size_t)n0 * K, (uint32_t)rows * K);
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-      const uint8_t* row = p.w + (size_t)min(n0 + 16 * i + fr, p.n - 1) * K + k;
+    for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-        s.w[i][h] = k + 64 * h < K ? *reinterpret_cast<const uint4*>(row + 64 * h) : make_uint4(0, 0, 0, 0);
-    }
-    s.ws = p.ws[(size_t)(n0 / kFp8Block) * nkb + kb];
+      for (int i = 0; i < R; i++)
+        s.w[i][h] = __builtin_amdgcn_raw_buffer_load_b128(
+            rs, ((16 * i + fr) * K + k + 64 * h) | (k + 64 * h < K ? 0 : (int)kDmaOut), 0, 0);
+    const int at = g < shape.groups ? ((n0 / kFp8Block) * nkb + kb) * 4 : (int)kDmaOut;
+    s.ws = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rt, at, 0, 0));
   };
   const int stride = (int)gridDim.x * kWideWaves;
   int g = (int)blockIdx.x * kWideWaves + wave;
+  const int blocks = g < shape.groups ? ((shape.groups - 1 - g) / stride + 1) * nkb : 0;  // of this wave
   Stage ring[D];
-#pragma unroll
-  for (int d = 0; d < D; d++)
-    if (g < shape.groups && d < nkb) load(ring[d], g, d);
+  int next_g = g, next_kb = 0;
+  auto load_next = [&](Stage& s) {
+    load(s, next_g, next_kb);
+    next_kb++;
+    next_g = next_kb == nkb ? next_g + stride : next_g;
+    next_kb = next_kb == nkb ? 0 : next_kb;
+  };
 
   // x: chunk c of a row's 128 bytes at c ^ (row % 8), so that the sixteen rows of
   // a fragment read spread over all banks; zeros behind the last row and column.
-  for (int c = tid; c < nkb * MB * 16 * 8; c += 64 * kWideWaves) {
-    const int kb = c / (MB * 16 * 8), row = c / 8 % (MB * 16), k = kb * kFp8Block + 16 * (c & 7);
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (row < p.m && k < K) v = *reinterpret_cast<const uint4*>(p.x + (size_t)row * K + k);
-    *reinterpret_cast<uint4*>(xl + ((size_t)kb * MB * 16 + row) * 128 + 16 * ((c & 7) ^ (row & 7))) = v;
+  // The matrix's first loads are issued behind x's last ones, which return first:
+  // in front of them, LDS would be filled only when the matrix has come.
+  constexpr int kChunks = 3 * MB, kStep = 64 * kWideWaves;
+  const __amdgpu_buffer_rsrc_t rx = read_rsrc(p.x, (uint32_t)p.m * K);
+  const __amdgpu_buffer_rsrc_t rxs = read_rsrc(p.xs, (uint32_t)(p.m * nkb) * 4u);
+  const int chunks = nkb * MB * 16 * 8;
+  u32x4 xv[kChunks];
+  auto load_x = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < kChunks; i++) {
+      const int c = c0 + i * kStep + tid, k = c / (MB * 16 * 8) * kFp8Block + 16 * (c & 7);
+      xv[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, (c / 8 % (MB * 16) * K + k) | (k < K ? 0 : (int)kDmaOut), 0, 0);
+    }
+  };
+  auto store_x = [&](int c0) {
+#pragma unroll
+    for (int i = 0; i < kChunks; i++) {
+      const int c = c0 + i * kStep + tid, row = c / 8;
+      if (c < chunks) *reinterpret_cast<u32x4*>(xl + (size_t)row * 128 + 16 * ((c & 7) ^ (row & 7))) = xv[i];
+    }
+  };
+  for (int c = tid; c < nkb * MB * 16; c += kStep) {
+    const int row = c % (MB * 16);
+    xsl[c] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+        rxs, row < p.m ? (row * nkb + c / (MB * 16)) * 4 : (int)kDmaOut, 0, 0));
   }
-  for (int c = tid; c < nkb * MB * 16; c += 64 * kWideWaves) {
-    const int kb = c / (MB * 16), row = c % (MB * 16);
-    xsl[c] = row < p.m ? p.xs[(size_t)row * nkb + kb] : 0.0f;
+  int c0 = 0;
+  for (; c0 + kChunks * kStep < chunks; c0 += kChunks * kStep) {
+    load_x(c0);
+    store_x(c0);
   }
+  load_x(c0);
+#pragma unroll
+  for (int d = 0; d < D; d++) load_next(ring[d]);
+  store_x(c0);
   __syncthreads();
 
   ScorePart sum[MB];
@@ -663,56 +712,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
       sum[j] = empty_part();
       token[j] = out.tokens && 16 * j + fr < p.m ? out.tokens[16 * j + fr] : -1;
     }
-  for (; g < shape.groups; g += stride) {
-    f32x4 acc[R][MB];
-#pragma unroll
-    for (int i = 0; i < R; i++)
-#pragma unroll
-      for (int j = 0; j < MB; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = 0; k0 < nkb; k0 += D) {
-#pragma unroll
-      for (int d = 0; d < D; d++) {
-        const int kb = k0 + d;
-        if (kb < nkb) {
-          const Stage& s = ring[d];
-          bf16x8 fw[R][4];
-#pragma unroll
-          for (int i = 0; i < R; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              fw[i][2 * h] = widen_fp8x8(s.w[i][h].x, s.w[i][h].y);
-              fw[i][2 * h + 1] = widen_fp8x8(s.w[i][h].z, s.w[i][h].w);
-            }
-          const char* xb = xl + (size_t)kb * MB * 16 * 128;
-#pragma unroll
-          for (int j = 0; j < MB; j++) {
-            const int row = 16 * j + fr;
-            bf16x8 fx[4];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint4 v = *reinterpret_cast<const uint4*>(xb + row * 128 + 16 * ((fg + 4 * h) ^ (row & 7)));
-              fx[2 * h] = widen_fp8x8(v.x, v.y);
-              fx[2 * h + 1] = widen_fp8x8(v.z, v.w);
-            }
-            const float sc = xsl[kb * MB * 16 + row] * s.ws;
-#pragma unroll
-            for (int i = 0; i < R; i++) {
-              f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-              for (int h = 0; h < 4; h++) v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i][h], fx[h], v, 0, 0, 0);
-#pragma unroll
-              for (int r = 0; r < 4; r++) acc[i][j][r] = fmaf(v[r], sc, acc[i][j][r]);
-            }
-          }
-        }
-        // The slot's next block: of this group, or behind its last blocks the next
-        // group's block d.
-        if (kb + D < nkb)
-          load(ring[d], g, kb + D);
-        else if (k0 + D >= nkb && d < nkb && g + stride < shape.groups)
-          load(ring[d], g + stride, d);
-      }
-    }
+  auto finish = [&](const f32x4 (&acc)[R][MB], int g) {
     const int n0 = g * kWideCols;
 #pragma unroll
     for (int j = 0; j < MB; j++) {
@@ -724,6 +724,58 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
       } else {
 #pragma unroll
         for (int i = 0; i < R; i++) store_columns<OUT>(p, out.y, 16 * j + fr, n0 + 16 * i + 4 * fg, acc[i][j]);
+      }
+    }
+  };
+  f32x4 acc[R][MB];
+#pragma unroll
+  for (int i = 0; i < R; i++)
+#pragma unroll
+    for (int j = 0; j < MB; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  int kb = 0;
+  for (int at = 0; at < blocks; at += D) {
+#pragma unroll
+    for (int d = 0; d < D; d++) {  // those past the last block multiply zeros
+      const Stage& s = ring[d];
+      bf16x8 fw[R][4];
+#pragma unroll
+      for (int i = 0; i < R; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          fw[i][2 * h] = widen_fp8x8(s.w[i][h].x, s.w[i][h].y);
+          fw[i][2 * h + 1] = widen_fp8x8(s.w[i][h].z, s.w[i][h].w);
+        }
+      const float ws = s.ws;
+      load_next(ring[d]);
+      const char* xb = xl + (size_t)kb * MB * 16 * 128;
+#pragma unroll
+      for (int j = 0; j < MB; j++) {
+        const int row = 16 * j + fr;
+        bf16x8 fx[4];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint4 v = *reinterpret_cast<const uint4*>(xb + row * 128 + 16 * ((fg + 4 * h) ^ (row & 7)));
+          fx[2 * h] = widen_fp8x8(v.x, v.y);
+          fx[2 * h + 1] = widen_fp8x8(v.z, v.w);
+        }
+        const float sc = xsl[kb * MB * 16 + row] * ws;
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+          f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int h = 0; h < 4; h++) v = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i][h], fx[h], v, 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; r++) acc[i][j][r] = fmaf(v[r], sc, acc[i][j][r]);
+        }
+      }
+      if (++kb == nkb) {
+        if (at + d < blocks) finish(acc, g);
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+          for (int j = 0; j < MB; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        kb = 0;
+        g += stride;
       }
     }
   }
