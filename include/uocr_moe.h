@@ -367,7 +367,10 @@ int uocr_fp8_quantize_weight(uocr_gpu_ctx* ctx, const void* w, uocr_dtype type, 
 /* y[m, n] = x . w^T of e4m3 rows x[m, k] with scales xs[m, ceil(k / 128)] and an
  * e4m3 matrix w[n, k] with scales ws[ceil(n / 128), ceil(k / 128)]; any finite
  * scales. Each block's products are summed and scaled in f32; y is F32 or BF16
- * (rounded once). A NaN byte makes its row or column NaN and raises nothing.
+ * (rounded once). BF16 results of more than 64 rows sum a block with the matrix
+ * cores' e4m3 instruction, which keeps 13 bits below the largest of every eight
+ * products (some 1e-5 of a sum, at most 2^-10 of the sum of magnitudes); F32 results
+ * keep all bits. A NaN byte makes its row or column NaN and raises nothing.
  * Equal calls give equal bits; a row's last bits depend on m, which chooses how
  * its sums are split. */
 int uocr_fp8_linear(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,

@@ -7,19 +7,9 @@
 // (src/cpu/quantized.rs:9-237); these stand beside its operators.
 #include <algorithm>
 
-#include "fp8.hpp"
-#include "mfma.hpp"
-#include "scores.hpp"
+#include "fp8_device.hpp"
 
 namespace uocr {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-// A raw buffer resource for loads: those at or past `bytes` give zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t read_rsrc(const void* base, uint32_t bytes) {
-  return store_rsrc(const_cast<void*>(base), bytes);
-}
 
 // ------------------------------------------------------------- quantisation
 
@@ -199,195 +189,6 @@ void launch_fp8_quantize_tiles(const void* x, int type, int rows, int cols, size
 
 // ------------------------------------------------------------------ product
 
-// What a product leaves: its values in f32 or bf16, or its rows' statistics.
-enum { kOutF32, kOutBf16, kOutScores };
-
-struct ProductOut {
-  void* y;              // [m, n]
-  ScorePart* parts;     // [column tiles][m]
-  const int32_t* tokens;
-  float* given;         // [m] logits of the given tokens
-};
-
-// Sixteen bytes of a row of K bytes from byte k, zeros behind the row's end.
-// Rows start at any address where K is not a multiple of 16.
-__device__ __forceinline__ uint4 load_chunk(const uint8_t* row, int k, int K) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (k + 16 <= K) {
-    __builtin_memcpy(&v, row + k, 16);
-  } else {
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 16; j++)
-      if (k + j < K) w[j / 4] |= (uint32_t)row[k + j] << (8 * (j & 3));
-    v = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  return v;
-}
-
-// Eight e4m3 values (two words) as bf16, which holds them exactly.
-__device__ __forceinline__ bf16x8 widen_fp8x8(uint32_t lo, uint32_t hi) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
-  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
-  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
-  return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
-// Four adjacent columns of row `row`, from column col on.
-template <int OUT>
-__device__ __forceinline__ void store_columns(const Fp8Product& p, void* y, int row, int col, f32x4 v) {
-  if (row >= p.m || col >= p.n) return;
-  const size_t at = (size_t)row * p.n + col;
-  if (p.n % 4 == 0) {  // four whole columns; y is aligned to its element, so is any of its rows to four
-    if (OUT == kOutF32) {
-      __builtin_memcpy(static_cast<float*>(y) + at, &v, 16);
-    } else {
-      const uint2 b = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
-      __builtin_memcpy(static_cast<uint16_t*>(y) + at, &b, 8);
-    }
-    return;
-  }
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    if (col + r >= p.n) return;
-    if (OUT == kOutF32)
-      static_cast<float*>(y)[at + r] = v[r];
-    else
-      static_cast<uint16_t*>(y)[at + r] = bf16_bits(v[r]);
-  }
-}
-
-// The statistics of one row's logits in a wave: lane l holds columns col + 16 i +
-// r of row l % 16 (v[i][r]; col differs between the four lanes of a row). Every
-// lane of the row gets them. The lane with the given token's column keeps its logit.
-template <int COUNT>
-__device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int col, int n, int token,
-                                                    float* given) {
-  ScorePart q = empty_part();
-  float most = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < COUNT; i++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int c = col + 16 * i + r;
-      if (c >= n) continue;
-      most = fmaxf(most, v[i][r]);
-      if (c == token) *given = v[i][r];
-    }
-  most = fmaxf(most, __shfl_xor(most, 16));
-  q.r = fmaxf(most, __shfl_xor(most, 32));
-#pragma unroll
-  for (int i = 0; i < COUNT; i++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      if (col + 16 * i + r >= n) continue;
-      const float d = (v[i][r] - q.r) * kLog2e;
-      const float e = __builtin_amdgcn_exp2f(d);
-      q.s += e;
-      q.t = fmaf(e, d, q.t);
-    }
-#pragma unroll
-  for (int o = 16; o <= 32; o <<= 1) {
-    q.s += __shfl_xor(q.s, o);
-    q.t += __shfl_xor(q.t, o);
-  }
-  return q;
-}
-
-// 128 x 128 outputs per workgroup of four waves, 64 x 64 each. The matrix cores'
-// e4m3 instructions bring each group of eight products to the largest one's
-// exponent and cut them off 13 bits below it (measured: 2^16 - 2^16 + v keeps
-// multiples of 8; 1.3e-5 of a Gaussian block's sum), so the operands are widened
-// to bf16, whose products are summed to f32's last bit (1e-8). One scale block is
-// a chain of four v_mfma_f32_16x16x32_bf16 from zero, scaled into the f32
-// accumulators when it is done. The matrix is the first operand: lane l then
-// holds four adjacent columns of y for row l % 16, whose x scale it needs as one
-// value.
-template <int OUT>
-__global__ __launch_bounds__(256) void fp8_tile_kernel(Fp8Product p, ProductOut out) {
-  constexpr int kT = 128;
-  __shared__ __attribute__((aligned(16))) uint8_t lds_w[kT * 128], lds_x[kT * 128];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int n0 = (int)blockIdx.x * kT, m0 = (int)blockIdx.y * kT;
-  const int wn = n0 + 64 * (wave & 1), wm = m0 + 64 * (wave >> 1);
-  const int fr = lane & 15, fg = lane >> 4;
-  const int K = p.k, nkb = p.kblocks();
-  f32x4 acc[4][4];  // [16 columns][16 rows]
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-
-  // Byte k of row r lies at chunk (k / 16) ^ (r % 8) of the row's 128 bytes:
-  // the sixteen rows of a fragment read then spread over all banks.
-  for (int kb = 0; kb < nkb; kb++) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const int chunk = tid + 256 * i, r = chunk >> 3, c = chunk & 7;
-      const int at = r * 128 + 16 * (c ^ (r & 7));
-      uint4 a = make_uint4(0, 0, 0, 0), b = a;
-      if (n0 + r < p.n) a = load_chunk(p.w + (size_t)(n0 + r) * K, kb * 128 + 16 * c, K);
-      if (m0 + r < p.m) b = load_chunk(p.x + (size_t)(m0 + r) * K, kb * 128 + 16 * c, K);
-      *reinterpret_cast<uint4*>(lds_w + at) = a;
-      *reinterpret_cast<uint4*>(lds_x + at) = b;
-    }
-    __syncthreads();
-    const float ws = p.ws[(size_t)(n0 / kFp8Block) * nkb + kb];
-    // Lane group g takes chunks g and g + 4 of both operands: the order of
-    // the 128 products inside a block is free.
-    struct Fragment {
-      bf16x8 part[4];
-    };
-    auto fragment = [&](const uint8_t* tile, int r) {
-      const uint4 lo = *reinterpret_cast<const uint4*>(tile + r * 128 + 16 * (fg ^ (r & 7)));
-      const uint4 hi = *reinterpret_cast<const uint4*>(tile + r * 128 + 16 * ((fg + 4) ^ (r & 7)));
-      return Fragment{{widen_fp8x8(lo.x, lo.y), widen_fp8x8(lo.z, lo.w), widen_fp8x8(hi.x, hi.y),
-                       widen_fp8x8(hi.z, hi.w)}};
-    };
-    Fragment fw[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) fw[i] = fragment(lds_w, wn - n0 + 16 * i + fr);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const Fragment fx = fragment(lds_x, wm - m0 + 16 * j + fr);
-      const int row = wm + 16 * j + fr;
-      const float sc = row < p.m ? p.xs[(size_t)row * nkb + kb] * ws : 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int h = 0; h < 4; h++) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i].part[h], fx.part[h], d, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; r++) acc[i][j][r] = fmaf(d[r], sc, acc[i][j][r]);
-      }
-    }
-  }
-
-  if constexpr (OUT == kOutScores) {
-    if (wn >= p.n) return;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int row = wm + 16 * j + fr;
-      const int token = out.tokens && row < p.m ? out.tokens[row] : -1;
-      const f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
-      const ScorePart q = row_statistics<4>(v, wn + 4 * fg, p.n, token, out.given + row);
-      if (fg == 0 && row < p.m) out.parts[(size_t)(wn / 64) * p.m + row] = q;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) store_columns<OUT>(p, out.y, wm + 16 * j + fr, wn + 16 * i + 4 * fg, acc[i][j]);
-  }
-}
-
-static dim3 tile_grid(const Fp8Product& p) {
-  return dim3((unsigned)((p.n + 127) / 128), (unsigned)((p.m + 127) / 128));
-}
-
 // ---- few rows (at most 64): the matrix is streamed from memory straight to the
 // registers of the wave that multiplies it, two scale blocks in flight; x comes
 // from the caches. A wave takes 16 RG columns of y (rows of the matrix) and all of
@@ -395,7 +196,6 @@ static dim3 tile_grid(const Fp8Product& p) {
 // add up in LDS, in order. Lane l reads the bytes [16 (l / 16), +16) and 64 bytes
 // on of row l % 16 in each block: a load instruction covers 64-byte runs.
 constexpr int kStreamRows = 64;
-constexpr int kCus = 256, kMostLds = 160 << 10;
 
 struct StreamShape {
   int ks, waves;  // waves that share a group's depth, waves per workgroup
@@ -527,7 +327,7 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
         f32x4 v[RG];
 #pragma unroll
         for (int i = 0; i < RG; i++) v[i] = acc[i][j];
-        const ScorePart q = row_statistics<RG>(v, n0 + 4 * fg, p.n, token, out.given + row);
+        const ScorePart q = row_statistics<RG>(v, n0, fg, p.n, token, out.given + row);
         if (fg == 0) held[slot * (16 * MB) + row] = n0 < p.n ? q : empty_part();
       }
     __syncthreads();
@@ -543,11 +343,6 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
 #pragma unroll
         for (int i = 0; i < RG; i++) store_columns<OUT>(p, out.y, 16 * j + fr, n0 + 16 * i + 4 * fg, acc[i][j]);
   }
-}
-
-// Whole 16-byte chunks of rows at aligned addresses.
-static bool whole_chunks(const Fp8Product& p) {
-  return p.k % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0;
 }
 
 static bool takes_stream(const Fp8Product& p) { return p.m <= kStreamRows && whole_chunks(p); }
@@ -720,7 +515,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
         f32x4 v[R];
 #pragma unroll
         for (int i = 0; i < R; i++) v[i] = acc[i][j];
-        sum[j] = join(sum[j], row_statistics<R>(v, n0 + 4 * fg, p.n, token[j], out.given + 16 * j + fr));
+        sum[j] = join(sum[j], row_statistics<R>(v, n0, fg, p.n, token[j], out.given + 16 * j + fr));
       } else {
 #pragma unroll
         for (int i = 0; i < R; i++) store_columns<OUT>(p, out.y, 16 * j + fr, n0 + 16 * i + 4 * fg, acc[i][j]);
@@ -816,6 +611,7 @@ void fp8_init_attributes() {
   wide_attributes<2>();
   wide_attributes<3>();
   wide_attributes<4>();
+  fp8_gemm_init_attributes();
   (void)hipGetLastError();  // a refused attribute surfaces at launch instead
 }
 
@@ -834,12 +630,8 @@ static void launch_product(const Fp8Product& p, const ProductOut& out, int kind,
   } else if (takes_stream(p)) {
     const StreamPlan t = plan_stream(p, kind == kOutScores);
     t.rg == 2 ? run_stream_rows<2>(p, out, kind, t, s) : run_stream_rows<1>(p, out, kind, t, s);
-  } else if (kind == kOutF32) {
-    fp8_tile_kernel<kOutF32><<<tile_grid(p), 256, 0, s>>>(p, out);
-  } else if (kind == kOutBf16) {
-    fp8_tile_kernel<kOutBf16><<<tile_grid(p), 256, 0, s>>>(p, out);
   } else {
-    fp8_tile_kernel<kOutScores><<<tile_grid(p), 256, 0, s>>>(p, out);
+    launch_fp8_gemm(p, out, kind, s);
   }
 }
 
@@ -851,14 +643,14 @@ void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, hipStream_t s) {
 
 // Parts per row.
 static int score_tiles(const Fp8Product& p) {
-  if (!takes_stream(p)) return (p.n + 63) / 64;
+  if (!takes_stream(p)) return fp8_gemm_parts(p);
   return takes_wide(p) ? kCus : plan_stream(p, true).grid;
 }
 
 size_t fp8_score_bytes(const Fp8Product& p) {
   // Room for p.m rows or fewer, whichever kernel takes them.
   const size_t few = std::min(p.m, kStreamRows);
-  return std::max((size_t)((p.n + 63) / 64) * p.m, (size_t)((p.n + 15) / 16) * few) * sizeof(ScorePart) +
+  return std::max((size_t)fp8_gemm_parts(p) * p.m, (size_t)((p.n + 15) / 16) * few) * sizeof(ScorePart) +
          (size_t)p.m * 4;
 }
 

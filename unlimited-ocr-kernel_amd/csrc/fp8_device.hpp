@@ -1,0 +1,123 @@
+// Device code shared by the e4m3 products (fp8.hip, fp8_gemm.hip).
+#pragma once
+
+#include "fp8.hpp"
+#include "mfma.hpp"
+#include "scores.hpp"
+
+namespace uocr {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// A raw buffer resource for loads: those at or past `bytes` give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t read_rsrc(const void* base, uint32_t bytes) {
+  return store_rsrc(const_cast<void*>(base), bytes);
+}
+
+constexpr int kCus = 256, kMostLds = 160 << 10;
+
+// What a product leaves: its values in f32 or bf16, or its rows' statistics.
+enum { kOutF32, kOutBf16, kOutScores };
+
+struct ProductOut {
+  void* y;              // [m, n]
+  ScorePart* parts;     // [column tiles][m]
+  const int32_t* tokens;
+  float* given;         // [m] logits of the given tokens
+};
+
+// Eight e4m3 values (two words) as bf16, which holds them exactly.
+__device__ __forceinline__ bf16x8 widen_fp8x8(uint32_t lo, uint32_t hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
+  return (bf16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Four adjacent columns of row `row`, from column col on.
+template <int OUT>
+__device__ __forceinline__ void store_columns(const Fp8Product& p, void* y, int row, int col, f32x4 v) {
+  if (row >= p.m || col >= p.n) return;
+  const size_t at = (size_t)row * p.n + col;
+  if (p.n % 4 == 0) {  // four whole columns; y is aligned to its element, so is any of its rows to four
+    if (OUT == kOutF32) {
+      __builtin_memcpy(static_cast<float*>(y) + at, &v, 16);
+    } else {
+      const uint2 b = make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+      __builtin_memcpy(static_cast<uint16_t*>(y) + at, &b, 8);
+    }
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    if (col + r >= p.n) return;
+    if (OUT == kOutF32)
+      static_cast<float*>(y)[at + r] = v[r];
+    else
+      static_cast<uint16_t*>(y)[at + r] = bf16_bits(v[r]);
+  }
+}
+
+// The statistics of one row's logits in a wave: lane l holds columns col + 16 i +
+// r of row l % 16 (v[i][r]; col differs by 4 between the four lanes of a row). Every
+// lane of the row gets them. The lane with the given token's column keeps its logit.
+// FULL: all of the columns are below n.
+template <int COUNT, bool FULL>
+__device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int col, int n, int token,
+                                                    float* given) {
+  ScorePart q = empty_part();
+  float most = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < COUNT; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) most = FULL || col + 16 * i + r < n ? fmaxf(most, v[i][r]) : most;
+  most = fmaxf(most, __shfl_xor(most, 16));
+  q.r = fmaxf(most, __shfl_xor(most, 32));
+#pragma unroll
+  for (int i = 0; i < COUNT; i++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const float d = FULL || col + 16 * i + r < n ? (v[i][r] - q.r) * kLog2e : -1000.0f;
+      const float e = __builtin_amdgcn_exp2f(d);
+      q.s += e;
+      q.t = fmaf(e, d, q.t);
+    }
+  const uint32_t off = (uint32_t)(token - col);
+  if (off < 16u * COUNT && (off & 12u) == 0 && token < n) {
+    float g = 0.0f;
+#pragma unroll
+    for (int i = 0; i < COUNT; i++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) g = off == 16u * i + r ? v[i][r] : g;
+    *given = g;
+  }
+#pragma unroll
+  for (int o = 16; o <= 32; o <<= 1) {
+    q.s += __shfl_xor(q.s, o);
+    q.t += __shfl_xor(q.t, o);
+  }
+  return q;
+}
+// The same, whether or not the wave's columns (from n0 on) end below n.
+template <int COUNT>
+__device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int n0, int fg, int n, int token,
+                                                    float* given) {
+  return n0 + 16 * COUNT <= n ? row_statistics<COUNT, true>(v, n0 + 4 * fg, n, token, given)
+                              : row_statistics<COUNT, false>(v, n0 + 4 * fg, n, token, given);
+}
+
+// fp8_gemm.hip: the product of many rows.
+// Parts per row that scores leave (ProductOut::parts), and the launch.
+int fp8_gemm_parts(const Fp8Product& p);
+void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s);
+void fp8_gemm_init_attributes();
+
+// Whole 16-byte chunks of rows at aligned addresses.
+inline bool whole_chunks(const Fp8Product& p) {
+  return p.k % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0;
+}
+
+}  // namespace uocr

@@ -55,37 +55,6 @@ __global__ void split_planes_kernel(const float* __restrict__ x, int rows, int K
         make_uint2(l[0] | ((uint32_t)l[1] << 16), l[2] | ((uint32_t)l[3] << 16));
 }
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-
-// Global -> LDS load that bypasses registers (buffer_load_dwordx4 ... lds):
-// lane l's 16 bytes land at LDS address M0 + 16 l, M0 being the wave-uniform
-// `lds_addr`. Range-checked like any raw buffer load: offsets at or past the
-// resource size write zeros. Written as inline assembly so the compiler does
-// not treat it as an LDS store to wait for before every LDS read; the
-// kernel waits on vmcnt itself before the barrier that publishes a stage.
-// M0 is reserved to the compiler, which uses it only for such LDS transfers
-// (none of its own here), so the asm sets it without declaring it.
-__device__ __forceinline__ void buffer_load_lds16(i32x4 rsrc, uint32_t lds_addr, uint32_t voffset) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(lds_addr), "v"(voffset), "s"(rsrc)
-               : "memory");
-}
-
-__device__ __forceinline__ i32x4 buffer_rsrc(const void* base, uint32_t bytes) {
-  const unsigned long long a = reinterpret_cast<unsigned long long>(base);
-  i32x4 r;
-  r.x = (int)(uint32_t)a;
-  r.y = (int)((a >> 32) & 0xffffu);  // stride 0
-  r.z = (int)bytes;
-  r.w = 0x00020000;  // gfx9 raw buffer word 3
-  return r;
-}
-
-// s_waitcnt immediate that waits for vmcnt <= n only (gfx9 encoding: vmcnt
-// bits [3:0] and [15:14], expcnt [6:4] and lgkmcnt [11:8] left at maximum).
-constexpr int vmcnt_only(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
-
 // One work item: a TM x TN output tile of group g, rows r0.. of the group,
 // columns n0... BF16 weights use two shapes: 256 x 256 (waves 2 x 4) for
 // groups with more than 128 rows left, and 128 x 512 (waves 1 x 8) for the

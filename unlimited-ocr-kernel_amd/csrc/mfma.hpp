@@ -46,4 +46,36 @@ __device__ __forceinline__ int vgpr_offset(int x) {
   return x;
 }
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// Global -> LDS load that bypasses registers (buffer_load_dwordx4 ... lds):
+// lane l's 16 bytes land at LDS address M0 + 16 l, M0 being the wave-uniform
+// `lds_addr`. Range-checked like any raw buffer load: offsets at or past the
+// resource size write zeros. Written as inline assembly so the compiler does
+// not treat it as an LDS store to wait for before every LDS read; the
+// kernel waits on vmcnt itself before the barrier that publishes a stage.
+// M0 is reserved to the compiler, which uses it only for such LDS transfers
+// (none of its own here), so the asm sets it without declaring it.
+__device__ __forceinline__ void buffer_load_lds16(i32x4 rsrc, uint32_t lds_addr, uint32_t voffset) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds_addr), "v"(voffset), "s"(rsrc)
+               : "memory");
+}
+
+__device__ __forceinline__ i32x4 buffer_rsrc(const void* base, uint32_t bytes) {
+  const unsigned long long a = reinterpret_cast<unsigned long long>(base);
+  i32x4 r;
+  r.x = (int)(uint32_t)a;
+  r.y = (int)((a >> 32) & 0xffffu);  // stride 0
+  r.z = (int)bytes;
+  r.w = 0x00020000;  // gfx9 raw buffer word 3
+  return r;
+}
+
+// s_waitcnt immediate that waits for vmcnt <= n only (gfx9 encoding: vmcnt
+// bits [3:0] and [15:14], expcnt [6:4] and lgkmcnt [11:8] left at maximum).
+constexpr int vmcnt_only(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
+
 }  // namespace uocr
