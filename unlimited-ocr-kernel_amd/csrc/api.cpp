@@ -1351,7 +1351,7 @@ void enqueue_product_scores(uocr_gpu_ctx* ctx, const uocr::Fp8Product& p, char* 
                             const uocr_token_scores& s, size_t row) {
   const uocr::TokenScores o = scores_from(s, row);
   if (s.n_top) {
-    uocr::launch_fp8_linear(p, work, uocr::kTypeF32, ctx->stream);
+    uocr::launch_fp8_linear(p, work, uocr::kTypeF32, nullptr, 0, ctx->stream);
     uocr::launch_token_scores(work, uocr::kTypeF32, p.m, p.n, p.n, o,
                               work + align256((size_t)p.m * p.n * 4), ctx->err, ctx->stream);
   } else {
@@ -1406,7 +1406,8 @@ int uocr_fp8_linear_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, 
   if (m == 0) return UOCR_OK;
   if (!y) return fail(UOCR_ERR_SHAPE, "null pointer");
   HIP_TRY(hipSetDevice(ctx->device), "set device");
-  uocr::launch_fp8_linear({x, xs, w, ws, (int)m, (int)n, (int)k}, y, ytype, ctx->stream);
+  uocr::launch_fp8_linear({x, xs, w, ws, (int)m, (int)n, (int)k}, y, ytype, ctx->scratch, ctx->scratch_limit,
+                          ctx->stream);
   HIP_TRY(hipGetLastError(), "kernel launch");
   return UOCR_OK;
 }
@@ -1611,7 +1612,7 @@ int uocr_lm_head_logits_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const
     const HeadRows rows = head_rows(ctx->scratch, v, 1);
     if (rows.bytes > ctx->scratch_limit) return scratch_fail(ctx);
     quantized_head_rows(ctx, v, last, 1, rows);
-    uocr::launch_fp8_linear(fp8_head(v, rows, 1), logits, uocr::kTypeF32, ctx->stream);
+    uocr::launch_fp8_linear(fp8_head(v, rows, 1), logits, uocr::kTypeF32, nullptr, 0, ctx->stream);
   } else if (uocr::lm_head_fast(v.H)) {
     uocr::launch_lm_head(last, v, logits, ctx->err, ctx->stream);
   } else {

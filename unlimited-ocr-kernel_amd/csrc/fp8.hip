@@ -620,7 +620,8 @@ static bool takes_wide(const Fp8Product& p) {
   return p.n >= kCus * kWideWaves * kWideCols && wide_lds(p) <= (size_t)kMostLds;
 }
 
-static void launch_product(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s) {
+static void launch_product(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
+                           hipStream_t s) {
   if (takes_stream(p) && takes_wide(p)) {
     const int mb = (p.m + 15) / 16;
     if (mb == 1) run_wide<1>(p, out, kind, s);
@@ -631,12 +632,12 @@ static void launch_product(const Fp8Product& p, const ProductOut& out, int kind,
     const StreamPlan t = plan_stream(p, kind == kOutScores);
     t.rg == 2 ? run_stream_rows<2>(p, out, kind, t, s) : run_stream_rows<1>(p, out, kind, t, s);
   } else {
-    launch_fp8_gemm(p, out, kind, s);
+    launch_fp8_gemm(p, out, kind, work, work_bytes, s);
   }
 }
 
-void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, hipStream_t s) {
-  launch_product(p, {y, nullptr, nullptr, nullptr}, ytype == kTypeF32 ? kOutF32 : kOutBf16, s);
+void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, void* work, size_t work_bytes, hipStream_t s) {
+  launch_product(p, {y, nullptr, nullptr, nullptr}, ytype == kTypeF32 ? kOutF32 : kOutBf16, work, work_bytes, s);
 }
 
 // ------------------------------------------------- scores from the product
@@ -705,7 +706,7 @@ void launch_fp8_scores(const Fp8Product& p, const TokenScores& out, void* work, 
   auto* parts = static_cast<ScorePart*>(work);
   auto* given = reinterpret_cast<float*>(parts + (size_t)tiles * p.m);
   const ProductOut po{nullptr, parts, out.logprobs ? out.tokens : nullptr, given};
-  launch_product(p, po, kOutScores, s);
+  launch_product(p, po, kOutScores, nullptr, 0, s);
 #define UOCR_JOIN(R)                                                                               \
   join_parts_kernel<R><<<(unsigned)((p.m + R - 1) / R), 64 * kJoinWaves, 0, s>>>(parts, tiles, p.m, p.n, \
                                                                                  given, out, err)

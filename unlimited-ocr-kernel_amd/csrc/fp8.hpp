@@ -33,7 +33,8 @@ struct Fp8Product {
   int m, n, k;
   __host__ __device__ int kblocks() const { return (k + kFp8Block - 1) / kFp8Block; }
 };
-void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, hipStream_t s);
+// `work`: room for partial sums where the depth is split; any size will do.
+void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, void* work, size_t work_bytes, hipStream_t s);
 
 // Scores of the product's rows without the logits in memory: partial
 // statistics per (column tile, row) and the given tokens' logits go to

@@ -112,7 +112,9 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
 // fp8_gemm.hip: the product of many rows.
 // Parts per row that scores leave (ProductOut::parts), and the launch.
 int fp8_gemm_parts(const Fp8Product& p);
-void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s);
+// `work` may be any size: without room for partial sums the depth is not split.
+void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
+                     hipStream_t s);
 void fp8_gemm_init_attributes();
 
 // Whole 16-byte chunks of rows at aligned addresses.

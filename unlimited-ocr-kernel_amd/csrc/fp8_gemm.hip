@@ -103,10 +103,9 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
   }
 }
 
-// ---- whole 16-byte chunks: TM x TN outputs per workgroup, 16 XB rows x 64 columns
-// per wave. A stage is one scale block deep: TM + TN rows of 128 bytes, brought by
-// global->LDS loads into one of two buffers while the other is multiplied. The
-// matrix is the matrix instruction's first operand: lane l then holds four adjacent
+// ---- whole 16-byte chunks: 128 x 128 outputs per workgroup of four waves, 64 x 64
+// each. A stage is one scale block deep: 256 rows of 128 bytes, brought by global->LDS
+// loads into a ring of buffers ahead of the one that is multiplied. The matrix is the matrix instruction's first operand: lane l then holds four adjacent
 // columns of y for row l % 16, whose x scale it needs as one value.
 //
 // WIDEN: the matrix cores' e4m3 instructions bring each group of eight products to
@@ -117,60 +116,96 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 // zero. bf16 results, rounded to 2^-9 anyway, take v_mfma_f32_16x16x128_f8f6f4, one
 // per scale block, at twice the rate. Either way a block's sum is scaled into the f32
 // accumulators when it is done.
-template <int WAVES_M, int WAVES_N, int XB_>
-struct TileShape {
-  static constexpr int kWm = WAVES_M, kWn = WAVES_N, kWaves = WAVES_M * WAVES_N, XB = XB_;
-  static constexpr int TM = WAVES_M * 16 * XB, TN = WAVES_N * 64;
-  static constexpr uint32_t kStage = (TM + TN) * 128u;
-  static constexpr size_t kLds = 2 * kStage;
+//
+// BUFS stages of LDS: with two, two workgroups share a CU and hide each other's waits
+// (many tiles); with four, one workgroup keeps three stages in flight (few tiles, where
+// the wait for memory is what counts). Few tiles of a long depth are also split along
+// it: each split leaves f32 partial sums in memory, and a second launch adds them in
+// order.
+constexpr int kTile = 128, kXb = 4;  // rows and columns of a tile, row blocks of a wave
+constexpr uint32_t kStage = 2 * kTile * 128u;
+// Scales of eight blocks: x's [8][kTile], the matrix's [8].
+constexpr uint32_t kScales = (8 * kTile + 8) * 4u;
+constexpr size_t tile_lds(int bufs) { return bufs * kStage + 2 * kScales; }
+
+// Workgroups reach the 8 XCDs round-robin, each XCD with an L2 of its own. They are
+// renumbered so that an XCD takes a contiguous run of tiles, and tiles run down strips
+// of kStrip row tiles: the tiles at work on an XCD at once are near square, so that
+// together they read the fewest rows of x and w.
+constexpr int kStrip = 8;
+struct TileAt {
+  int m, n;
+};
+__device__ __forceinline__ TileAt tile_of(int id, int tiles_m, int tiles_n) {
+  const int total = tiles_m * tiles_n, xcd = id % kXcds, each = total / kXcds, more = total % kXcds;
+  const int at = xcd * each + min(xcd, more) + id / kXcds;
+  const int strip = at / (kStrip * tiles_n), in = at % (kStrip * tiles_n);
+  const int rows = min(kStrip, tiles_m - strip * kStrip);
+  return {strip * kStrip + in % rows, in / rows};
+}
+
+// Blocks [split * each, + each) of the depth; a split's results go to its own [m, n]
+// of y.
+struct Splits {
+  int count, each;
 };
 
-template <class S, bool WIDEN, int OUT>
-__global__ __launch_bounds__(64 * S::kWaves, 2) void fp8_tile_kernel(Fp8Product p, ProductOut out) {
-  constexpr int XB = S::XB, TM = S::TM, TN = S::TN;
+template <bool WIDEN, int OUT, int BUFS>
+__global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductOut out, Splits splits) {
+  constexpr int XB = kXb;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, fg = lane >> 4;
   const int K = p.k, nkb = p.kblocks();
-  const int m0 = (int)blockIdx.y * TM, n0 = (int)blockIdx.x * TN;
-  const int wm = wave / S::kWn * (16 * XB), wn = wave % S::kWn * 64;
+  const int tiles_m = (p.m + kTile - 1) / kTile, tiles_n = (p.n + kTile - 1) / kTile;
+  // The splits of a tile lie far apart: an XCD works on neighbouring tiles at one depth.
+  const int split = (int)blockIdx.x / (tiles_m * tiles_n);
+  const TileAt tile = tile_of((int)blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n);
+  const int first = split * splits.each, last = min(nkb, first + splits.each);
+  const int m0 = tile.m * kTile, n0 = tile.n * kTile;
+  const int wm = wave / 2 * 64, wn = wave % 2 * 64;
 
   // Loads: a wave instruction brings 8 rows of 128 bytes; chunk c of row r lies at c
   // ^ (r % 8), which spreads a fragment read's sixteen rows over all banks.
-  constexpr int kSegX = TM / 8 / S::kWaves, kSegW = TN / 8 / S::kWaves;
-  const i32x4 rx = buffer_rsrc(p.x + (size_t)m0 * K, (uint32_t)min(TM, p.m - m0) * K);
-  const i32x4 rw = buffer_rsrc(p.w + (size_t)n0 * K, (uint32_t)min(TN, p.n - n0) * K);
+  constexpr int kSegs = kTile / 8 / 4, kLoads = 2 * kSegs;
+  const i32x4 rx = buffer_rsrc(p.x + (size_t)m0 * K, (uint32_t)min(kTile, p.m - m0) * K);
+  const i32x4 rw = buffer_rsrc(p.w + (size_t)n0 * K, (uint32_t)min(kTile, p.n - n0) * K);
   const int chunk = (lane & 7) ^ (lane >> 3);
-  const uint32_t xat = (uint32_t)(wave * kSegX * 8 + (lane >> 3)) * K + 16 * chunk;
-  const uint32_t wat = (uint32_t)(wave * kSegW * 8 + (lane >> 3)) * K + 16 * chunk;
+  const uint32_t at = (uint32_t)(wave * kSegs * 8 + (lane >> 3)) * K + 16 * chunk;
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
-  auto issue = [&](int buf, int kb) {
+  auto issue = [&](int kb) {
     const uint32_t k = (uint32_t)kb * 128u;
     const uint32_t past = (int)k + 16 * chunk < K ? 0u : kDmaOut;
-    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)buf * S::kStage);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(kb % BUFS) * kStage);
 #pragma unroll
-    for (int i = 0; i < kSegX; i++)
-      buffer_load_lds16(rx, to + (uint32_t)(wave * kSegX + i) * 1024u, (xat + (uint32_t)(8 * i) * K + k) | past);
-#pragma unroll
-    for (int i = 0; i < kSegW; i++)
-      buffer_load_lds16(rw, to + TM * 128u + (uint32_t)(wave * kSegW + i) * 1024u,
-                        (wat + (uint32_t)(8 * i) * K + k) | past);
+    for (int i = 0; i < kSegs; i++) {
+      const uint32_t off = (at + (uint32_t)(8 * i) * K + k) | past;
+      buffer_load_lds16(rx, to + (uint32_t)(wave * kSegs + i) * 1024u, off);
+      buffer_load_lds16(rw, to + kTile * 128u + (uint32_t)(wave * kSegs + i) * 1024u, off);
+    }
   };
-  // Scales of the wave's rows (lane l: row l % 16 of each block) and of its columns,
-  // which lie in one tile of the matrix.
-  const __amdgpu_buffer_rsrc_t rxs = read_rsrc(p.xs + (size_t)m0 * nkb, (uint32_t)(min(TM, p.m - m0) * nkb) * 4u);
-  const __amdgpu_buffer_rsrc_t rws =
-      read_rsrc(p.ws, (uint32_t)((p.n + kFp8Block - 1) / kFp8Block * nkb) * 4u);
-  const int wsat = (n0 + wn) / kFp8Block * nkb;
+  // Scales of eight blocks at a time, in LDS beside the stages. A thread brings four
+  // blocks of one row of x (16 bytes; a lane per row and block, 4 bytes each of a line
+  // of its own, took as long as the stages), some one of the matrix's.
+  const __amdgpu_buffer_rsrc_t rxs = read_rsrc(p.xs + (size_t)m0 * nkb, (uint32_t)(min(kTile, p.m - m0) * nkb) * 4u);
+  const __amdgpu_buffer_rsrc_t rws = read_rsrc(p.ws + (size_t)tile.n * nkb, (uint32_t)nkb * 4u);
   struct Scales {
-    float x[XB], w;
+    u32x4 x;
+    uint32_t w;
   };
-  auto load_scales = [&](Scales& s, int kb) {
+  auto load_scales = [&](int eighth) {  // blocks past the last one: anything
+    Scales s;
+    s.x = __builtin_amdgcn_raw_buffer_load_b128(rxs, ((tid >> 1) * nkb + 8 * eighth + 4 * (tid & 1)) * 4, 0, 0);
+    s.w = __builtin_amdgcn_raw_buffer_load_b32(rws, (8 * eighth + (tid & 7)) * 4, 0, 0);
+    return s;
+  };
+  auto scales_at = [&](int eighth) { return reinterpret_cast<float*>(lds + BUFS * kStage + (eighth & 1) * kScales); };
+  auto store_scales = [&](int eighth, const Scales& s) {
+    float* to = scales_at(eighth);
 #pragma unroll
-    for (int j = 0; j < XB; j++)
-      s.x[j] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rxs, ((wm + 16 * j + fr) * nkb + kb) * 4, 0, 0));
-    s.w = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rws, (wsat + kb) * 4, 0, 0));
+    for (int i = 0; i < 4; i++) to[(4 * (tid & 1) + i) * kTile + (tid >> 1)] = __uint_as_float(s.x[i]);
+    if (tid < 8) to[8 * kTile + tid] = __uint_as_float(s.w);
   };
 
   f32x4 acc[4][XB];
@@ -183,85 +218,120 @@ __global__ __launch_bounds__(64 * S::kWaves, 2) void fp8_tile_kernel(Fp8Product 
   };
   // Lane group g takes chunks g and g + 4 of both operands: the order of the 128
   // products inside a block is free.
-  struct Wide {
-    bf16x8 part[4];
+  struct Raw {
+    u32x4 half[2];
   };
-  auto widen = [&](u32x4 lo, u32x4 hi) {
-    return Wide{{widen_fp8x8(lo.x, lo.y), widen_fp8x8(lo.z, lo.w), widen_fp8x8(hi.x, hi.y), widen_fp8x8(hi.z, hi.w)}};
-  };
-  auto join8 = [&](u32x4 lo, u32x4 hi) {
-    return (i32x8){(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
-  };
-  auto multiply = [&](int buf, const Scales& s) {
-    const char* xt = lds + (size_t)buf * S::kStage;
-    const char* wt = xt + TM * 128;
-    if constexpr (WIDEN) {
-      Wide fw[4];
+  auto read = [&](const char* tile, int r) { return Raw{{chunk_at(tile, r, fg), chunk_at(tile, r, fg + 4)}}; };
+  // One stage. While row block j is multiplied, block j - 1's sums are scaled, block
+  // j + 1's fragment is widened and block j + 2's is read; the order within a step is
+  // held by sched_barrier. Left to itself the compiler waits for each product before
+  // it scales it.
+  auto scale = [&](f32x4& a, const f32x4& d, float sc) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int r = wn + 16 * i + fr;
-        fw[i] = widen(chunk_at(wt, r, fg), chunk_at(wt, r, fg + 4));
-      }
+    for (int r = 0; r < 4; r++) a[r] = fmaf(d[r], sc, a[r]);
+    asm volatile("" : "+v"(a));  // here, not sunk behind the loop's next branch
+  };
+  auto multiply = [&](int kb) {
+    const char* xt = lds + (size_t)(kb % BUFS) * kStage;
+    const char* wt = xt + kTile * 128;
+    const float* xs = scales_at(kb >> 3) + (kb & 7) * kTile + wm + fr;
+    const float ws = scales_at(kb >> 3)[8 * kTile + (kb & 7)];
+    float sc[2];
+    f32x4 d[2][4];
+    auto zero = [&](f32x4 (&v)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    };
+    if constexpr (WIDEN) {
+      // Eight values of a fragment: half h / 2's words 2 (h % 2) and 2 (h % 2) + 1.
+      auto part = [&](const Raw& v, int h) { return widen_fp8x8(v.half[h / 2][2 * (h & 1)], v.half[h / 2][2 * (h & 1) + 1]); };
+      Raw rw4[4], raw[2];
+      bf16x8 fw[4][4], fx[2][4];
+      raw[0] = read(xt, wm + fr);
+#pragma unroll
+      for (int i = 0; i < 4; i++) rw4[i] = read(wt, wn + 16 * i + fr);
+      if (XB > 1) raw[1] = read(xt, wm + 16 + fr);
+#pragma unroll
+      for (int h = 0; h < 4; h++) fx[0][h] = part(raw[0], h);
+#pragma unroll
+      for (int h = 0; h < 4; h++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) fw[i][h] = part(rw4[i], h);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < XB; j++) {
-        const int r = wm + 16 * j + fr;
-        const Wide fx = widen(chunk_at(xt, r, fg), chunk_at(xt, r, fg + 4));
-        const float sc = s.x[j] * s.w;
-        f32x4 d[4];
+        if (j + 2 < XB) raw[j & 1] = read(xt, wm + 16 * (j + 2) + fr);
+        sc[j & 1] = xs[16 * j] * ws;
+        zero(d[j & 1]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) d[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int h = 0; h < 4; h++)
+        for (int h = 0; h < 4; h++) {
 #pragma unroll
           for (int i = 0; i < 4; i++)
-            d[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i].part[h], fx.part[h], d[i], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int r4 = 0; r4 < 4; r4++) acc[i][j][r4] = fmaf(d[i][r4], sc, acc[i][j][r4]);
+            d[j & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i][h], fx[j & 1][h], d[j & 1][i], 0, 0, 0);
+          if (j + 1 < XB) fx[(j + 1) & 1][h] = part(raw[(j + 1) & 1], h);
+          if (j > 0) scale(acc[h][j - 1], d[(j - 1) & 1][h], sc[(j - 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     } else {
-      i32x8 fw[4];
+      auto whole = [&](const Raw& v) {
+        return (i32x8){(int)v.half[0].x, (int)v.half[0].y, (int)v.half[0].z, (int)v.half[0].w,
+                       (int)v.half[1].x, (int)v.half[1].y, (int)v.half[1].z, (int)v.half[1].w};
+      };
+      Raw fw[4], fx[2];
+      fx[0] = read(xt, wm + fr);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int r = wn + 16 * i + fr;
-        fw[i] = join8(chunk_at(wt, r, fg), chunk_at(wt, r, fg + 4));
-      }
+      for (int i = 0; i < 4; i++) fw[i] = read(wt, wn + 16 * i + fr);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int j = 0; j < XB; j++) {
-        const int r = wm + 16 * j + fr;
-        const i32x8 fx = join8(chunk_at(xt, r, fg), chunk_at(xt, r, fg + 4));
-        const float sc = s.x[j] * s.w;
+        if (j + 1 < XB) fx[(j + 1) & 1] = read(xt, wm + 16 * (j + 1) + fr);
+        sc[j & 1] = xs[16 * j] * ws;
+        zero(d[j & 1]);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-          const f32x4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw[i], fx, zero, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-          for (int r4 = 0; r4 < 4; r4++) acc[i][j][r4] = fmaf(d[r4], sc, acc[i][j][r4]);
+          d[j & 1][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(whole(fw[i]), whole(fx[j & 1]), d[j & 1][i], 0,
+                                                                         0, 0, 0, 0, 0);
+          if (j > 0) scale(acc[i][j - 1], d[(j - 1) & 1][i], sc[(j - 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
+#pragma unroll
+    for (int i = 0; i < 4; i++) scale(acc[i][XB - 1], d[(XB - 1) & 1][i], sc[(XB - 1) & 1]);
   };
 
-  Scales now, next;
-  issue(0, 0);
-  load_scales(now, 0);
-  __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
-  __syncthreads();
-  for (int kb = 0; kb < nkb; kb++) {
-    if (kb + 1 < nkb) {
-      issue((kb + 1) & 1, kb + 1);
-      load_scales(next, kb + 1);
-    }
-    multiply(kb & 1, now);
-    now = next;
-    __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
+  // Stage kb is multiplied while the BUFS - 1 behind it are on their way. A wave's loads
+  // return in order, so its own part of stage kb is there when at most those of the
+  // later stages are outstanding; the barrier then publishes every wave's, and says
+  // that stage kb - 1, whose buffer the next loads fill, has been read.
+  constexpr int kAhead = BUFS - 1;
+  Scales next = load_scales(first >> 3);
+  for (int i = 0; i < kAhead; i++)
+    if (first + i < last) issue(first + i);
+  store_scales(first >> 3, next);
+  next = load_scales((first >> 3) + 1);
+  for (int kb = first; kb < last; kb++) {
+    if (kb + kAhead <= last)
+      __builtin_amdgcn_s_waitcnt(vmcnt_only((kAhead - 1) * kLoads));
+    else
+      __builtin_amdgcn_s_waitcnt(vmcnt_only(0));
     __syncthreads();
+    if (kb + kAhead < last) issue(kb + kAhead);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(kb);
+    __builtin_amdgcn_sched_barrier(0);
+    // The other eight blocks' scales were last read a step or more ago.
+    if ((kb & 7) == 7) {
+      store_scales((kb >> 3) + 1, next);
+      next = load_scales((kb >> 3) + 2);
+    }
   }
 
   if constexpr (OUT == kOutScores) {
-    // One part per tile and row: the columns' waves join in LDS.
+    // One part per tile and row: the two waves of a row join in LDS.
     ScorePart* held = reinterpret_cast<ScorePart*>(lds);
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < XB; j++) {
       const int r = wm + 16 * j + fr, row = m0 + r;
@@ -269,46 +339,102 @@ __global__ __launch_bounds__(64 * S::kWaves, 2) void fp8_tile_kernel(Fp8Product 
       const f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
       ScorePart q = empty_part();
       if (n0 + wn < p.n) q = row_statistics<4>(v, n0 + wn, fg, p.n, token, out.given + row);
-      if (fg == 0) held[wave % S::kWn * TM + r] = q;
+      if (fg == 0) held[wave % 2 * kTile + r] = q;
     }
     __syncthreads();
-    for (int r = tid; r < TM && m0 + r < p.m; r += 64 * S::kWaves) {
-      ScorePart q = held[r];
-      for (int w = 1; w < S::kWn; w++) q = join(q, held[w * TM + r]);
-      out.parts[(size_t)blockIdx.x * p.m + m0 + r] = q;
-    }
+    if (tid < kTile && m0 + tid < p.m)
+      out.parts[(size_t)tile.n * p.m + m0 + tid] = join(held[tid], held[kTile + tid]);
   } else {
+    char* y = static_cast<char*>(out.y) + (size_t)split * p.m * p.n * (OUT == kOutF32 ? 4 : 2);
 #pragma unroll
     for (int j = 0; j < XB; j++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        store_columns<OUT>(p, out.y, m0 + wm + 16 * j + fr, n0 + wn + 16 * i + 4 * fg, acc[i][j]);
+        store_columns<OUT>(p, y, m0 + wm + 16 * j + fr, n0 + wn + 16 * i + 4 * fg, acc[i][j]);
   }
 }
 
-using Tile256 = TileShape<2, 4, 8>;
-using Tile128 = TileShape<2, 2, 4>;
-
-template <class S, bool WIDEN, int OUT>
-static void run_tiles(const Fp8Product& p, const ProductOut& out, hipStream_t s) {
-  const dim3 grid((unsigned)((p.n + S::TN - 1) / S::TN), (unsigned)((p.m + S::TM - 1) / S::TM));
-  fp8_tile_kernel<S, WIDEN, OUT><<<grid, 64 * S::kWaves, S::kLds, s>>>(p, out);
+// Adds the splits' partial sums in order.
+template <int OUT>
+__global__ __launch_bounds__(256) void add_splits_kernel(const float* __restrict__ parts, size_t count, int splits,
+                                                         void* __restrict__ y) {
+  const size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= count) return;
+  if (i + 4 <= count) {
+    f32x4 a;
+    __builtin_memcpy(&a, parts + i, 16);
+#pragma unroll 4
+    for (int s = 1; s < splits; s++) {
+      f32x4 b;
+      __builtin_memcpy(&b, parts + s * count + i, 16);
+#pragma unroll
+      for (int r = 0; r < 4; r++) a[r] += b[r];
+    }
+    if (OUT == kOutF32) {
+      __builtin_memcpy(static_cast<float*>(y) + i, &a, 16);
+    } else {
+      const uint2 b = make_uint2(bf16_pair(a[0], a[1]), bf16_pair(a[2], a[3]));
+      __builtin_memcpy(static_cast<uint16_t*>(y) + i, &b, 8);
+    }
+    return;
+  }
+  for (size_t e = i; e < count; e++) {
+    float a = parts[e];
+    for (int s = 1; s < splits; s++) a += parts[s * count + e];
+    if (OUT == kOutF32)
+      static_cast<float*>(y)[e] = a;
+    else
+      static_cast<uint16_t*>(y)[e] = bf16_bits(a);
+  }
 }
 
-using ScoreTile = Tile128;
+template <bool WIDEN, int OUT, int BUFS>
+static void run_tiles(const Fp8Product& p, const ProductOut& out, const Splits& splits, hipStream_t s) {
+  const unsigned tiles = (unsigned)((p.n + kTile - 1) / kTile) * (unsigned)((p.m + kTile - 1) / kTile);
+  fp8_tile_kernel<WIDEN, OUT, BUFS><<<tiles * splits.count, 256, tile_lds(BUFS), s>>>(p, out, splits);
+}
+
+// Two workgroups per CU need twice as many tiles as there are CUs.
+static bool many_tiles(const Fp8Product& p) {
+  return (size_t)((p.n + kTile - 1) / kTile) * ((p.m + kTile - 1) / kTile) > (size_t)kCus;
+}
+
+// How many ways to split the depth: by a model of the time in units of 0.1 us, with what
+// was measured for its parts: a step of a workgroup that has a CU to itself 6, a round of
+// workgroups' start and end 30, the second launch 25 and its traffic 5 GB/ms each way.
+static Splits plan_splits(const Fp8Product& p, size_t work_bytes) {
+  const int nkb = p.kblocks();
+  Splits best{1, nkb};
+  if (many_tiles(p)) return best;
+  const size_t tiles = (size_t)((p.n + kTile - 1) / kTile) * ((p.m + kTile - 1) / kTile), bytes = (size_t)p.m * p.n * 4;
+  double least = 1e30;
+  for (int each = nkb; each >= 2; each--) {
+    const int count = (nkb + each - 1) / each;
+    if (count > 1 && count * bytes > work_bytes) break;
+    const double rounds = (double)((tiles * count + kCus - 1) / kCus);
+    const double time = rounds * (30 + 6.0 * each) + (count > 1 ? 25 + 2.0 * count * bytes / 5e5 : 0.0);
+    if (time < least) {
+      least = time;
+      best = {count, each};
+    }
+  }
+  return best;
+}
 
 int fp8_gemm_parts(const Fp8Product& p) {
-  return whole_chunks(p) ? (p.n + ScoreTile::TN - 1) / ScoreTile::TN : (p.n + 63) / 64;
+  return whole_chunks(p) ? (p.n + kTile - 1) / kTile : (p.n + 63) / 64;
 }
 
 void fp8_gemm_init_attributes() {
-  const void* kernels[] = {(const void*)fp8_tile_kernel<Tile256, false, kOutBf16>,
-                           (const void*)fp8_tile_kernel<Tile128, true, kOutF32>,
-                           (const void*)fp8_tile_kernel<ScoreTile, true, kOutScores>};
+  const void* kernels[] = {(const void*)fp8_tile_kernel<false, kOutBf16, 2>, (const void*)fp8_tile_kernel<false, kOutBf16, 4>,
+                           (const void*)fp8_tile_kernel<false, kOutF32, 4>, (const void*)fp8_tile_kernel<true, kOutF32, 2>,
+                           (const void*)fp8_tile_kernel<true, kOutF32, 4>, (const void*)fp8_tile_kernel<true, kOutScores, 2>,
+                           (const void*)fp8_tile_kernel<true, kOutScores, 4>};
   for (const void* k : kernels) (void)hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
 }
 
-void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s) {
+void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
+                     hipStream_t s) {
   if (!whole_chunks(p)) {
     const dim3 grid((unsigned)((p.n + 127) / 128), (unsigned)((p.m + 127) / 128));
     if (kind == kOutF32)
@@ -317,12 +443,31 @@ void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, hipSt
       fp8_bytes_kernel<kOutBf16><<<grid, 256, 0, s>>>(p, out);
     else
       fp8_bytes_kernel<kOutScores><<<grid, 256, 0, s>>>(p, out);
-  } else if (kind == kOutF32) {
-    run_tiles<Tile128, true, kOutF32>(p, out, s);
-  } else if (kind == kOutBf16) {
-    run_tiles<Tile256, false, kOutBf16>(p, out, s);
+    return;
+  }
+  const bool many = many_tiles(p);
+  const Splits one{1, p.kblocks()};
+  if (kind == kOutScores) {
+    many ? run_tiles<true, kOutScores, 2>(p, out, one, s) : run_tiles<true, kOutScores, 4>(p, out, one, s);
+    return;
+  }
+  const Splits splits = plan_splits(p, work_bytes);
+  if (splits.count == 1) {
+    if (kind == kOutF32)
+      many ? run_tiles<true, kOutF32, 2>(p, out, one, s) : run_tiles<true, kOutF32, 4>(p, out, one, s);
+    else
+      many ? run_tiles<false, kOutBf16, 2>(p, out, one, s) : run_tiles<false, kOutBf16, 4>(p, out, one, s);
+    return;
+  }
+  const ProductOut parts{work, nullptr, nullptr, nullptr};
+  const size_t count = (size_t)p.m * p.n;
+  const unsigned grid = (unsigned)((count + 1023) / 1024);
+  if (kind == kOutF32) {
+    run_tiles<true, kOutF32, 4>(p, parts, splits, s);
+    add_splits_kernel<kOutF32><<<grid, 256, 0, s>>>((const float*)work, count, splits.count, out.y);
   } else {
-    run_tiles<ScoreTile, true, kOutScores>(p, out, s);
+    run_tiles<false, kOutF32, 4>(p, parts, splits, s);
+    add_splits_kernel<kOutBf16><<<grid, 256, 0, s>>>((const float*)work, count, splits.count, out.y);
   }
 }
 
