@@ -171,7 +171,12 @@ __device__ __forceinline__ unsigned long long block_max(unsigned long long key,
 // Groups and candidates that the short way holds; more (many equal logits) take
 // the long one, which passes over the row once for each alternative.
 constexpr int kMostGroups = 512, kMostCandidates = 1024;
+// Group maxima that a thread keeps in registers (rows of up to 131072 or 262144
+// logits); those of longer rows are read twice.
+constexpr int kHeldMaxima = 8;
 
+// A chain of dependent reads (the maxima; then the candidates' logits) and barriers,
+// which is what it takes: everything that can be read early is.
 template <typename T>
 __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     const T* __restrict__ logits, int vocab, size_t ld, int chunks,
@@ -181,14 +186,23 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   __shared__ ScorePart held[kScoreThreads / 64];
   __shared__ unsigned long long keys[kMostCandidates];
   __shared__ int listed[kMostGroups];
-  __shared__ float mine[kScoreThreads];
-  __shared__ float tau_at;
+  __shared__ __attribute__((aligned(16))) float mine[kScoreThreads];
+  __shared__ uint32_t tau_at;
   __shared__ int counts[2];
   const size_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int token = out.tokens ? out.tokens[row] : 0;
   const int top = out.top;
-  if (token < 0) {  // a padding row
+  const float* gmax = maxima + row * groups;
+  float g[kHeldMaxima];
+#pragma unroll
+  for (int i = 0; i < kHeldMaxima; i++) {
+    const int at = tid + i * kScoreThreads;
+    g[i] = top && at < groups ? gmax[at] : -INFINITY;
+  }
+  ScorePart p = empty_part();
+  for (int c = tid; c < chunks; c += kScoreThreads) p = join(p, parts[row * chunks + c]);
+  const int token = out.tokens ? out.tokens[row] : 0;
+  if (token < 0) {  // a padding row; what was read of it is not used
     if (tid == 0 && out.logprobs) out.logprobs[row] = 0.0f;
     if (tid == 0 && out.entropy) out.entropy[row] = 0.0f;
     for (int i = tid; i < top; i += kScoreThreads) {
@@ -198,28 +212,36 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     return;
   }
   const T* x = logits + row * ld;
-  const float* gmax = maxima + row * groups;
   const float given = tid == 0 && out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f;
-  ScorePart p = empty_part();
-  for (int c = tid; c < chunks; c += kScoreThreads) p = join(p, parts[row * chunks + c]);
   // This thread's largest group.
-  float most = -INFINITY;
+  float most = g[0];
+#pragma unroll
+  for (int i = 1; i < kHeldMaxima; i++) most = fmaxf(most, g[i]);
   if (top)
-    for (int g = tid; g < groups; g += kScoreThreads) most = fmaxf(most, gmax[g]);
+    for (int at = tid + kHeldMaxima * kScoreThreads; at < groups; at += kScoreThreads) most = fmaxf(most, gmax[at]);
+  // tau is chosen from as few maxima as there may be alternatives: of four, two or
+  // single threads each.
+  const int share = top <= 16 ? 4 : top <= 32 ? 2 : 1;
+  if (share >= 2) most = fmaxf(most, dpp_move<0xB1>(most));
+  if (share == 4) most = fmaxf(most, dpp_move<0x4E>(most));
+  if (tid % share == 0) mine[tid / share] = most;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) p = join(p, shfl_xor(p, o));
   if (lane == 0) held[wave] = p;
-  // Up to sixteen alternatives need 64 maxima to choose tau from: four lanes' each.
-  const int many = top <= 16 ? kScoreThreads / 4 : kScoreThreads;
-  if (top <= 16) {
-    most = fmaxf(most, dpp_move<0xB1>(most));
-    most = fmaxf(most, dpp_move<0x4E>(most));
-    if ((tid & 3) == 0) mine[tid >> 2] = most;
-  } else {
-    mine[tid] = most;
-  }
   if (tid < 2) counts[tid] = 0;
+  if (tid == 0) tau_at = ~0u;
   __syncthreads();
+  // The n-th largest is the least of those that fewer than n are larger than.
+  const int many = kScoreThreads / share;
+  if (top && tid < many) {
+    const float v = mine[tid];
+    int larger = 0;
+    for (int i = 0; i < many; i += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(mine + i);
+      larger += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
+    }
+    if (larger < top) atomicMin(&tau_at, (uint32_t)(order_key(v, 0) >> 32));
+  }
   p = join(join(held[0], held[1]), join(held[2], held[3]));
   if (tid == 0) write_scores(out, row, token, vocab, p, given, err);
   if (top == 0) return;
@@ -230,33 +252,40 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     }
     return;
   }
-  if (tid < many) {
-    const float v = mine[tid];
-    int before = 0;
-    for (int i = 0; i < many; i++) before += mine[i] > v || (mine[i] == v && i < tid);
-    if (before == top - 1) tau_at = v;
-  }
   __syncthreads();
-  const float tau = tau_at;
+  const float tau = key_value((unsigned long long)tau_at << 32);
   // With tau -inf (fewer finite logits than alternatives, or nearly): all finite
   // logits, and the first columns' banned ones to fill up with.
   const bool finite = tau > -INFINITY;
-  for (int g = tid; g < groups; g += kScoreThreads)
-    if (finite ? gmax[g] >= tau : gmax[g] > -INFINITY || g == 0) {
-      const int at = atomicAdd(&counts[0], 1);
-      if (at < kMostGroups) listed[at] = g;
-    }
+  auto list = [&](int at, float v) {
+    if (at >= groups || !(finite ? v >= tau : v > -INFINITY || at == 0)) return;
+    const int to = atomicAdd(&counts[0], 1);
+    if (to < kMostGroups) listed[to] = at;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeldMaxima; i++) list(tid + i * kScoreThreads, g[i]);
+  for (int at = tid + kHeldMaxima * kScoreThreads; at < groups; at += kScoreThreads) list(at, gmax[at]);
   __syncthreads();
   const int some = counts[0];
   if (some <= kMostGroups) {
-    for (int i = tid; i < some * kGroup; i += kScoreThreads) {
-      const int col = listed[i / kGroup] * kGroup + i % kGroup;
-      if (col >= vocab) continue;
-      const float v = Logits<T>::widen(x[col]);
-      if (finite ? v >= tau : v > -INFINITY || col < top) {
-        const int at = atomicAdd(&counts[1], 1);
-        if (at < kMostCandidates) keys[at] = order_key(v, (uint32_t)col);
-      }
+    // Sixteen threads to a group, a vector each; two groups' loads in flight.
+    auto consider = [&](int c, const float (&v)[kVec]) {
+#pragma unroll
+      for (int j = 0; j < kVec; j++)
+        if (c + j < vocab && (finite ? v[j] >= tau : v[j] > -INFINITY || c + j < top)) {
+          const int to = atomicAdd(&counts[1], 1);
+          if (to < kMostCandidates) keys[to] = order_key(v[j], (uint32_t)(c + j));
+        }
+    };
+    constexpr int kPass = kScoreThreads / 16;
+    for (int i = tid / 16; i < some; i += 2 * kPass) {
+      const int ca = listed[i] * kGroup + (tid & 15) * kVec;
+      const int cb = i + kPass < some ? listed[i + kPass] * kGroup + (tid & 15) * kVec : vocab;
+      float a[kVec], b[kVec];
+      load_logits<T>(x, ca, vocab, a);
+      load_logits<T>(x, cb, vocab, b);
+      consider(ca, a);
+      consider(cb, b);
     }
     __syncthreads();
   }

@@ -437,7 +437,7 @@ class LmHead:
         arguments)."""
         s = _token_scores(hidden.shape[0], tokens, logprobs, entropy, top_ids, top_logprobs)
         _check(_operator("uocr_lm_head_logprobs", sync)(ctx.handle, self.handle, _ptr(hidden),
-                                                        hidden.shape[0], ctypes.byref(s)))
+                                                        hidden.shape[0], s))
 
     @property
     def precision(self) -> str:
@@ -508,67 +508,74 @@ def rms_norm(ctx: Context, x, weight, eps: float, out):
 FP8_BLOCK = 128
 MAX_TOP = 64
 
-
-def _shape(ok: bool, message: str):
-    if not ok:
-        raise UocrError(SHAPE, message)
+# These checks stand between a tensor and its address, and cost a short call
+# more than its kernel: one condition per operand.
 
 
-def _blocks(n: int) -> int:
-    return -(-n // FP8_BLOCK)
+def _refuse(message: str, status: int = SHAPE):
+    raise UocrError(status, message)
 
 
-_TYPES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}
+_types = {}
 
 
 def _type(t) -> int:
     """uocr_dtype of a floating torch tensor (others: Unsupported)."""
-    code = _TYPES.get(str(t.dtype))
+    code = _types.get(t.dtype)
     if code is None:
-        raise UocrError(UNSUPPORTED, f"element type {t.dtype}")
+        code = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}.get(str(t.dtype))
+        if code is None:
+            _refuse(f"element type {t.dtype}", UNSUPPORTED)
+        _types[t.dtype] = code
     return code
 
 
-def _rows(t, what: str) -> int:
-    """The row stride of a 2-D tensor whose rows are contiguous."""
-    _shape(t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), f"{what} must be rows")
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+def _rows(t, what: str):
+    """(rows, columns, row stride) of a 2-D tensor whose rows are contiguous."""
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+        _refuse(f"{what} must be rows")
+    rows, cols = t.shape
+    return rows, cols, t.stride(0) if rows > 1 else max(cols, 1)
 
 
-def _quantize(name, ctx, x, q, scales, scale_rows, sync):
-    ld = _rows(x, "x")
-    rows, cols = x.shape
-    _shape(tuple(q.shape) == (rows, cols) and q.is_contiguous() and q.element_size() == 1,
-           "q must be contiguous bytes of x's shape")
-    _shape(tuple(scales.shape) == (scale_rows, _blocks(cols)) and scales.is_contiguous(),
-           "scales must be one per block")
-    _check(_operator(name, sync)(ctx.handle, x.data_ptr(), _type(x), rows, cols, ld,
-                                 q.data_ptr(), scales.data_ptr()))
+def _quantize(fn, ctx, x, q, scales, tile: int):
+    rows, cols, ld = _rows(x, "x")
+    if q.shape != (rows, cols) or q.element_size() != 1 or not q.is_contiguous():
+        _refuse("q must be contiguous bytes of x's shape")
+    if scales.shape != (-(-rows // tile), -(-cols // 128)) or scales.element_size() != 4 \
+            or not scales.is_contiguous():
+        _refuse("scales must be one per block")
+    status = fn(ctx.handle, x.data_ptr(), _type(x), rows, cols, ld, q.data_ptr(),
+                scales.data_ptr())
+    if status:
+        _check(status)
 
 
 def fp8_quantize(ctx: Context, x, q, scales, sync: bool = True):
     """Rows x [rows, cols] (f32 or bf16, any row stride) to e4m3 q [rows, cols]
     (float8_e4m3fn or uint8) and f32 scales [rows, ceil(cols / 128)]."""
-    _quantize("uocr_fp8_quantize", ctx, x, q, scales, x.shape[0], sync)
+    _quantize(_operator("uocr_fp8_quantize", sync), ctx, x, q, scales, 1)
 
 
 def fp8_quantize_weight(ctx: Context, w, q, scales):
     """A matrix w [rows, cols] to e4m3 with scales [ceil(rows / 128),
     ceil(cols / 128)], one per 128 x 128 tile."""
-    _quantize("uocr_fp8_quantize_weight", ctx, w, q, scales, _blocks(w.shape[0]), True)
+    _quantize(_operator("uocr_fp8_quantize_weight"), ctx, w, q, scales, FP8_BLOCK)
 
 
 def _product(xq, xs, wq, ws):
     """The product's arguments (uocr_fp8_linear's second to eighth)."""
-    _shape(xq.dim() == 2 and wq.dim() == 2 and xq.shape[1] == wq.shape[1],
-           "x [m, k] and w [n, k] must agree")
+    if xq.dim() != 2 or wq.dim() != 2 or xq.shape[1] != wq.shape[1]:
+        _refuse("x [m, k] and w [n, k] must agree")
     m, k = xq.shape
     n = wq.shape[0]
-    _shape(tuple(xs.shape) == (m, _blocks(k)) and tuple(ws.shape) == (_blocks(n), _blocks(k)),
-           "scales must be [m, blocks(k)] and [blocks(n), blocks(k)]")
-    _shape(xq.is_contiguous() and wq.is_contiguous() and xs.is_contiguous() and ws.is_contiguous()
-           and xq.element_size() == 1 and wq.element_size() == 1 and xs.element_size() == 4
-           and ws.element_size() == 4, "product operands must be contiguous e4m3 and f32")
+    blocks = -(-k // 128)
+    if xs.shape != (m, blocks) or ws.shape != (-(-n // 128), blocks):
+        _refuse("scales must be [m, blocks(k)] and [blocks(n), blocks(k)]")
+    if not (xq.is_contiguous() and wq.is_contiguous() and xs.is_contiguous()
+            and ws.is_contiguous() and xq.element_size() == 1 and wq.element_size() == 1
+            and xs.element_size() == 4 and ws.element_size() == 4):
+        _refuse("product operands must be contiguous e4m3 and f32")
     return xq.data_ptr(), xs.data_ptr(), m, k, wq.data_ptr(), ws.data_ptr(), n
 
 
@@ -576,19 +583,28 @@ def fp8_linear(ctx: Context, xq, xs, wq, ws, y, sync: bool = True):
     """y [m, n] (f32 or bf16) = x . w^T of e4m3 rows xq [m, k] with scales xs and
     an e4m3 matrix wq [n, k] with scales ws per 128 x 128 tile."""
     args = _product(xq, xs, wq, ws)
-    _shape(tuple(y.shape) == (args[2], args[6]) and y.is_contiguous(), "y must be [m, n]")
-    _check(_operator("uocr_fp8_linear", sync)(ctx.handle, *args, y.data_ptr(), _type(y)))
+    if y.shape != (args[2], args[6]) or not y.is_contiguous():
+        _refuse("y must be [m, n]")
+    status = _operator("uocr_fp8_linear", sync)(ctx.handle, *args, y.data_ptr(), _type(y))
+    if status:
+        _check(status)
+
+
+def _score_address(t, shape):
+    if t is None:
+        return None
+    if t.shape != shape or t.element_size() != 4 or not t.is_contiguous():
+        _refuse("score arrays must be contiguous 32-bit values, one per row (and alternative)")
+    return t.data_ptr()
 
 
 def _token_scores(rows, tokens, logprobs, entropy, top_ids, top_logprobs) -> TokenScores:
-    n_top = top_ids.shape[1] if top_ids is not None else 0
-    for t, shape, size in ((tokens, (rows,), 4), (logprobs, (rows,), 4), (entropy, (rows,), 4),
-                           (top_ids, (rows, n_top), 4), (top_logprobs, (rows, n_top), 4)):
-        _shape(t is None or (tuple(t.shape) == shape and t.is_contiguous()
-                             and t.element_size() == size),
-               "score arrays must be contiguous 32-bit values, one per row (and alternative)")
-    return TokenScores(_ptr(tokens), n_top, _ptr(logprobs), _ptr(entropy), _ptr(top_ids),
-                       _ptr(top_logprobs))
+    one = (rows,)
+    n_top = 0 if top_ids is None else top_ids.shape[-1]
+    top = (rows, n_top)
+    return TokenScores(_score_address(tokens, one), n_top, _score_address(logprobs, one),
+                       _score_address(entropy, one), _score_address(top_ids, top),
+                       _score_address(top_logprobs, top))
 
 
 def token_logprobs(ctx: Context, logits, tokens=None, logprobs=None, entropy=None, top_ids=None,
@@ -597,11 +613,12 @@ def token_logprobs(ctx: Context, logits, tokens=None, logprobs=None, entropy=Non
     probability of tokens [rows] (int32; negative: a padding row), the entropy,
     and the most probable ids top_ids [rows, n] (int32) with their log
     probabilities. Outputs are f32 tensors to fill; None skips one."""
-    ld = _rows(logits, "logits")
-    rows, vocab = logits.shape
+    rows, vocab, ld = _rows(logits, "logits")
     s = _token_scores(rows, tokens, logprobs, entropy, top_ids, top_logprobs)
-    _check(_operator("uocr_token_logprobs", sync)(ctx.handle, logits.data_ptr(), _type(logits),
-                                                  rows, vocab, ld, ctypes.byref(s)))
+    status = _operator("uocr_token_logprobs", sync)(ctx.handle, logits.data_ptr(), _type(logits),
+                                                    rows, vocab, ld, s)
+    if status:
+        _check(status)
 
 
 def fp8_linear_logprobs(ctx: Context, xq, xs, wq, ws, tokens=None, logprobs=None, entropy=None,
@@ -610,7 +627,9 @@ def fp8_linear_logprobs(ctx: Context, xq, xs, wq, ws, tokens=None, logprobs=None
     unless alternatives are asked for."""
     args = _product(xq, xs, wq, ws)
     s = _token_scores(args[2], tokens, logprobs, entropy, top_ids, top_logprobs)
-    _check(_operator("uocr_fp8_linear_logprobs", sync)(ctx.handle, *args, ctypes.byref(s)))
+    status = _operator("uocr_fp8_linear_logprobs", sync)(ctx.handle, *args, s)
+    if status:
+        _check(status)
 
 
 # --------------------------------------------------------------- files
