@@ -283,6 +283,19 @@ def test_linear_random(ctx, m, n, k):
     assert (off <= tol + 2.0 ** -8 * (np.abs(want) + tol)).all()
 
 
+# More than 64 rows of products too small for the tiles: 64 rows to a workgroup, the
+# last ones with 1 to 64, and depths shared by up to sixteen waves.
+MANY_SMALL = [(65, 33, 16), (65, 1300, 896), (100, 700, 272), (129, 2100, 1296), (191, 16, 640), (200, 1, 128),
+              (300, 130, 6848), (1000, 17, 400), (2049, 65, 144)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY_SMALL)
+def test_linear_many_rows_of_small_products(ctx, m, n, k):
+    say(f"small product {m}x{n}x{k}")
+    test_linear_exact(ctx, m, n, k)
+    test_linear_random(ctx, m, n, k)
+
+
 def device_exact(m, n, k, seed):
     """exact_product made on the device, with its result there in float64."""
     g = torch.Generator(device="cuda")
@@ -304,7 +317,11 @@ def device_exact(m, n, k, seed):
 # Vocabularies: whole and ragged columns and depths, x small and too large for LDS.
 @pytest.mark.parametrize("m,n,k", [(1, 65536, 1280), (1, 129280, 1280), (3, 70001, 272), (16, 65549, 128),
                                    (17, 66000, 144), (33, 129280, 640), (48, 65600, 1280), (64, 65537, 1296),
-                                   (64, 65700, 2400), (1, 66000, 6848), (5, 65530, 16)])
+                                   (64, 65700, 2400), (1, 66000, 6848), (5, 65530, 16),
+                                   # More tiles than fit the card at once; depths of one, two and
+                                   # many blocks, and of more than eight.
+                                   (2100, 5001, 112), (1500, 6848, 272), (1300, 8000, 1296),
+                                   (130, 66000, 400), (4096, 2052, 2192)])
 def test_linear_wide_exact(ctx, m, n, k):
     say(f"wide product {m}x{n}x{k}")
     ops, want = device_exact(m, n, k, m + n)

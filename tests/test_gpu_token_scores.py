@@ -314,8 +314,16 @@ def test_linear_logprobs_random(ctx, m, n, k):
     assert all(np.array_equal(out.host()[x], again.host()[x]) for x in out.host())
 
 
+@pytest.mark.parametrize("m,n,k", [(65, 33, 16), (100, 700, 272), (129, 2100, 1296), (200, 1, 128),
+                                   (300, 130, 6848), (2049, 65, 144)])
+def test_linear_logprobs_many_rows_of_small_products(ctx, m, n, k):
+    say(f"small fused scores {m}x{n}x{k}")
+    test_linear_logprobs_exact_logits(ctx, m, n, k)
+    test_linear_logprobs_random(ctx, m, n, k)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 129280, 1280), (2, 65536, 144), (19, 70001, 256), (48, 66003, 640),
-                                   (64, 65700, 2400)])
+                                   (64, 65700, 2400), (1100, 8200, 272), (700, 20000, 1296)])
 def test_linear_logprobs_wide(ctx, m, n, k):
     say(f"wide fused scores {m}x{n}x{k}")
     (x, xs, w, ws), logits = device_exact(m, n, k, m + n)

@@ -189,13 +189,20 @@ void launch_fp8_quantize_tiles(const void* x, int type, int rows, int cols, size
 
 // ------------------------------------------------------------------ product
 
-// ---- few rows (at most 64): the matrix is streamed from memory straight to the
-// registers of the wave that multiplies it, two scale blocks in flight; x comes
-// from the caches. A wave takes 16 RG columns of y (rows of the matrix) and all of
-// x's rows, as MB blocks of 16; KS waves of a workgroup share a group's depth and
-// add up in LDS, in order. Lane l reads the bytes [16 (l / 16), +16) and 64 bytes
-// on of row l % 16 in each block: a load instruction covers 64-byte runs.
+// ---- few rows: the matrix is streamed from memory straight to the registers of the
+// wave that multiplies it, two scale blocks in flight; x comes from the caches. A wave
+// takes 16 RG columns of y (rows of the matrix) and up to 64 of x's rows, as MB blocks of
+// 16 (more rows: more workgroups, in the grid's second dimension); KS waves of a
+// workgroup share a group's depth and add up in LDS, in order. Lane l reads the bytes
+// [16 (l / 16), +16) and 64 bytes on of row l % 16 in each block: a load instruction
+// covers 64-byte runs.
+// More than 64 rows stay here while rows (whole 64) x columns x scale blocks are at
+// most kStreamMost, where the tiles' fewer workgroups leave most of the card idle.
+// Time on tiles over time here, bf16 / f32 results: at 1 to 2 Mi 1.1 to 2.1; at 4 Mi
+// 0.86 / 1.18 (512 x 1280 x 896), 1.27 / 1.85 (512 x 896 x 1280), 1.17 / 1.31 (128 x
+// 2560 x 1792); at 8 Mi 0.62 to 0.77 / 0.85 to 1.11; beyond 16 Mi the tiles win.
 constexpr int kStreamRows = 64;
+constexpr size_t kStreamMost = (size_t)4 << 20;
 
 struct StreamShape {
   int ks, waves;  // waves that share a group's depth, waves per workgroup
@@ -205,14 +212,20 @@ struct StreamShape {
 constexpr int kStreamDepth = 2;
 // Most waves of a workgroup, by the registers that a wave then may have: 128 where
 // x has one or two blocks of rows and a wave one group of columns, 256 otherwise.
-constexpr int stream_waves(int mb, int rg) { return rg == 1 ? (mb <= 2 ? 16 : 8) : 4; }
+constexpr int stream_waves(int mb, int rg) { return rg == 1 && mb <= 2 ? 16 : 8; }
 
 template <int MB, int RG, int OUT>
-__global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kernel(Fp8Product p, ProductOut out, StreamShape shape) {
+__global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kernel(Fp8Product p, ProductOut out,
+                                                                                  StreamShape shape) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, fg = lane >> 4;
+  // This workgroup's rows become the product's.
+  const int m0 = (int)blockIdx.y * kStreamRows, rows = p.m;
+  p.x += (size_t)m0 * p.k;
+  p.xs += (size_t)m0 * p.kblocks();
+  p.m = min(kStreamRows, rows - m0);
   const int groups = shape.waves / shape.ks;  // of this workgroup
   const int slot = wave / shape.ks, k0 = wave % shape.ks;
   const int n0 = ((int)blockIdx.x * groups + slot) * 16 * RG;
@@ -323,51 +336,57 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
 #pragma unroll
       for (int j = 0; j < MB; j++) {
         const int row = 16 * j + fr;
-        const int token = out.tokens && row < p.m ? out.tokens[row] : -1;
+        const int token = out.tokens && row < p.m ? out.tokens[m0 + row] : -1;
         f32x4 v[RG];
 #pragma unroll
         for (int i = 0; i < RG; i++) v[i] = acc[i][j];
-        const ScorePart q = row_statistics<RG>(v, n0, fg, p.n, token, out.given + row);
+        const ScorePart q = row_statistics<RG>(v, n0, fg, p.n, token, out.given + m0 + row);
         if (fg == 0) held[slot * (16 * MB) + row] = n0 < p.n ? q : empty_part();
       }
     __syncthreads();
     if (tid < 16 * MB && tid < p.m) {
       ScorePart q = held[tid];
       for (int g = 1; g < groups; g++) q = join(q, held[g * (16 * MB) + tid]);
-      out.parts[(size_t)blockIdx.x * p.m + tid] = q;
+      out.parts[(size_t)blockIdx.x * rows + m0 + tid] = q;
     }
   } else {
+    char* y = static_cast<char*>(out.y) + (size_t)m0 * p.n * (OUT == kOutF32 ? 4 : 2);
     if (k0 == 0)
 #pragma unroll
       for (int j = 0; j < MB; j++)
 #pragma unroll
-        for (int i = 0; i < RG; i++) store_columns<OUT>(p, out.y, 16 * j + fr, n0 + 16 * i + 4 * fg, acc[i][j]);
+        for (int i = 0; i < RG; i++) store_columns<OUT>(p, y, 16 * j + fr, n0 + 16 * i + 4 * fg, acc[i][j]);
   }
 }
 
-static bool takes_stream(const Fp8Product& p) { return p.m <= kStreamRows && whole_chunks(p); }
+static bool takes_stream(const Fp8Product& p) {
+  if (!whole_chunks(p)) return false;
+  const size_t rows = (size_t)(p.m + kStreamRows - 1) / kStreamRows * kStreamRows;
+  return p.m <= kStreamRows || rows * (size_t)p.n * p.kblocks() <= kStreamMost;
+}
 
 struct StreamPlan {
   int rg, mb;
   StreamShape shape;
-  int grid;
+  dim3 grid;
   size_t lds;
 };
 static StreamPlan plan_stream(const Fp8Product& p, bool scores) {
   StreamPlan s;
-  s.mb = (p.m + 15) / 16;
-  s.rg = (p.n + 31) / 32 >= 2048 ? 2 : 1;
+  const int chunks = (p.m + kStreamRows - 1) / kStreamRows;
+  s.mb = (std::min(p.m, kStreamRows) + 15) / 16;
+  s.rg = (p.n + 31) / 32 * chunks >= (chunks > 1 ? 128 : 2048) ? 2 : 1;
   const int groups = (p.n + 16 * s.rg - 1) / (16 * s.rg);
   // Waves of a group: as many as fill the card, then as few as leave each the same
   // whole rounds of kStreamDepth blocks.
-  const int want = std::min({stream_waves(s.mb, s.rg), p.kblocks(), (2048 + groups - 1) / groups});
+  const int want = std::min({stream_waves(s.mb, s.rg), p.kblocks(), (2048 + groups * chunks - 1) / (groups * chunks)});
   int each = (p.kblocks() + want - 1) / want;
   each = (each + kStreamDepth - 1) / kStreamDepth * kStreamDepth;
   const int ks = (p.kblocks() + each - 1) / each;
   const int per = std::max(1, 4 / ks);
   s.shape.ks = ks;
   s.shape.waves = per * ks;
-  s.grid = (groups + per - 1) / per;
+  s.grid = dim3((unsigned)((groups + per - 1) / per), (unsigned)chunks);
   s.lds = ks > 1 ? (size_t)s.shape.waves * s.rg * s.mb * 64 * sizeof(f32x4) : 0;
   if (scores) s.lds = std::max(s.lds, (size_t)per * 16 * s.mb * sizeof(ScorePart));
   return s;
@@ -375,7 +394,7 @@ static StreamPlan plan_stream(const Fp8Product& p, bool scores) {
 
 template <int MB, int RG>
 static void run_stream(const Fp8Product& p, const ProductOut& out, int kind, const StreamPlan& t, hipStream_t s) {
-  const dim3 grid(t.grid), block(64 * t.shape.waves);
+  const dim3 grid = t.grid, block(64 * t.shape.waves);
   if (kind == kOutF32)
     fp8_stream_kernel<MB, RG, kOutF32><<<grid, block, t.lds, s>>>(p, out, t.shape);
   else if (kind == kOutBf16)
@@ -617,12 +636,12 @@ void fp8_init_attributes() {
 
 // Enough columns to keep every wave at work, and x fits into LDS.
 static bool takes_wide(const Fp8Product& p) {
-  return p.n >= kCus * kWideWaves * kWideCols && wide_lds(p) <= (size_t)kMostLds;
+  return p.m <= kStreamRows && whole_chunks(p) && p.n >= kCus * kWideWaves * kWideCols && wide_lds(p) <= (size_t)kMostLds;
 }
 
 static void launch_product(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
                            hipStream_t s) {
-  if (takes_stream(p) && takes_wide(p)) {
+  if (takes_wide(p)) {
     const int mb = (p.m + 15) / 16;
     if (mb == 1) run_wide<1>(p, out, kind, s);
     if (mb == 2) run_wide<2>(p, out, kind, s);
@@ -645,13 +664,14 @@ void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, void* work, size
 // Parts per row.
 static int score_tiles(const Fp8Product& p) {
   if (!takes_stream(p)) return fp8_gemm_parts(p);
-  return takes_wide(p) ? kCus : plan_stream(p, true).grid;
+  return takes_wide(p) ? kCus : (int)plan_stream(p, true).grid.x;
 }
 
 size_t fp8_score_bytes(const Fp8Product& p) {
   // Room for p.m rows or fewer, whichever kernel takes them.
-  const size_t few = std::min(p.m, kStreamRows);
-  return std::max((size_t)fp8_gemm_parts(p) * p.m, (size_t)((p.n + 15) / 16) * few) * sizeof(ScorePart) +
+  const size_t most = kStreamMost / ((size_t)p.n * p.kblocks()) / kStreamRows * kStreamRows;
+  const size_t streamed = std::min<size_t>(p.m, std::max<size_t>(most, kStreamRows));
+  return std::max((size_t)fp8_gemm_parts(p) * p.m, (size_t)((p.n + 15) / 16) * streamed) * sizeof(ScorePart) +
          (size_t)p.m * 4;
 }
 

@@ -75,12 +75,17 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
 #pragma unroll
     for (int r = 0; r < 4; r++) most = FULL || col + 16 * i + r < n ? fmaxf(most, v[i][r]) : most;
   most = fmaxf(most, __shfl_xor(most, 16));
-  q.r = fmaxf(most, __shfl_xor(most, 32));
+  most = fmaxf(most, __shfl_xor(most, 32));
+  // d = log2(e) x - r2 in one instruction; r2's rounding, the same for all of the row's
+  // logits here, is put right at the end (2^c = 1 + c ln 2 for a c of some 1e-6).
+  // Logits past 1e38, whose r2 would overflow, end as an infinite sum.
+  q.r = fminf(fmaxf(most, -1e38f), 1e38f);
+  const float r2 = q.r * kLog2e;
 #pragma unroll
   for (int i = 0; i < COUNT; i++)
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const float d = FULL || col + 16 * i + r < n ? (v[i][r] - q.r) * kLog2e : -1000.0f;
+      const float d = FULL || col + 16 * i + r < n ? fmaf(v[i][r], kLog2e, -r2) : -1000.0f;
       const float e = __builtin_amdgcn_exp2f(d);
       q.s += e;
       q.t = fmaf(e, d, q.t);
@@ -99,6 +104,10 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
     q.s += __shfl_xor(q.s, o);
     q.t += __shfl_xor(q.t, o);
   }
+  const float c = fmaf(-q.r, kLog2e, r2);
+  q.t = fmaf(q.s, c, q.t);
+  q.t = fmaf(q.t, c * kLn2, q.t);
+  q.s = fmaf(q.s, c * kLn2, q.s);
   return q;
 }
 // The same, whether or not the wave's columns (from n0 on) end below n.

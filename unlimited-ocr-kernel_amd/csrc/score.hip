@@ -219,9 +219,10 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   for (int i = 1; i < kHeldMaxima; i++) most = fmaxf(most, g[i]);
   if (top)
     for (int at = tid + kHeldMaxima * kScoreThreads; at < groups; at += kScoreThreads) most = fmaxf(most, gmax[at]);
-  // tau is chosen from as few maxima as there may be alternatives: of four, two or
-  // single threads each.
-  const int share = top <= 16 ? 4 : top <= 32 ? 2 : 1;
+  // tau is chosen from the maxima of four, two or single threads each: fewer to rank,
+  // as long as they are as many as the alternatives.
+  const int filled = min(groups, kScoreThreads);
+  const int share = 4 * top <= filled ? 4 : 2 * top <= filled ? 2 : 1;
   if (share >= 2) most = fmaxf(most, dpp_move<0xB1>(most));
   if (share == 4) most = fmaxf(most, dpp_move<0x4E>(most));
   if (tid % share == 0) mine[tid / share] = most;
