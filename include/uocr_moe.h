@@ -367,12 +367,14 @@ int uocr_fp8_quantize_weight(uocr_gpu_ctx* ctx, const void* w, uocr_dtype type, 
 /* y[m, n] = x . w^T of e4m3 rows x[m, k] with scales xs[m, ceil(k / 128)] and an
  * e4m3 matrix w[n, k] with scales ws[ceil(n / 128), ceil(k / 128)]; any finite
  * scales. Each block's products are summed and scaled in f32; y is F32 or BF16
- * (rounded once). BF16 results of more than 64 rows sum a block with the matrix
- * cores' e4m3 instruction, which keeps 13 bits below the largest of every eight
- * products (some 1e-5 of a sum, at most 2^-10 of the sum of magnitudes); F32 results
- * keep all bits. A NaN byte makes its row or column NaN and raises nothing.
- * Equal calls give equal bits; a row's last bits depend on m, which chooses how
- * its sums are split. */
+ * (rounded once). BF16 results of more than 64 rows may sum a block with the
+ * matrix cores' e4m3 instruction, which keeps 13 bits below the largest of every
+ * eight products (some 1e-5 of a sum, at most 2^-10 of the sum of magnitudes);
+ * F32 results keep all bits. A NaN byte makes its row or column NaN and raises
+ * nothing. Works in the context's scratch: long depths of few rows and columns are
+ * split, as far as the partial sums fit. Equal calls give equal bits; a row's last
+ * bits depend on m and on the scratch limit, which choose how its sums are split.
+ * m, n and k are at most 2^22 (Resource). */
 int uocr_fp8_linear(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
                     const uint8_t* w, const float* ws, size_t n, void* y, uocr_dtype ytype);
 int uocr_fp8_linear_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
@@ -407,9 +409,10 @@ int uocr_token_logprobs(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype type, 
 int uocr_token_logprobs_async(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype type, size_t rows,
                               size_t vocab, size_t ld, const uocr_token_scores* scores);
 /* Scores of the rows of uocr_fp8_linear's product. With n_top 0 the logits stay
- * in registers (scratch: some 16 bytes per row and 256 ids); alternatives take
- * them through the context's scratch in f32, as many rows at a time as fit
- * (none: Resource). A logit that is not finite raises Numerical. */
+ * in registers (scratch: 16 bytes per row and 128 ids, for at most 64 rows per 16
+ * ids); alternatives take them through the context's scratch in f32, as many rows
+ * at a time as fit (none: Resource). A row with a logit that is not finite gets
+ * NaN and raises Numerical; logits in registers may do so from 1e38 on. */
 int uocr_fp8_linear_logprobs(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m,
                              size_t k, const uint8_t* w, const float* ws, size_t n,
                              const uocr_token_scores* scores);
@@ -450,7 +453,8 @@ int uocr_lm_head_logits_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const
  * with FP32 rows (W8A8 only where T == 1 under DynamicActivations). FP8 heads
  * quantise each normalised row and score it as uocr_fp8_linear_logprobs does;
  * the others hold logits in the context's scratch, as many rows at a time as
- * fit. T == 0 is a no-op. */
+ * fit. The hidden rows of padding tokens are not looked at either. T == 0 is a
+ * no-op. */
 int uocr_lm_head_logprobs(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,
                           size_t T, const uocr_token_scores* scores);
 int uocr_lm_head_logprobs_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const float* hidden,

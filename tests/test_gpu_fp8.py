@@ -286,7 +286,8 @@ def test_linear_random(ctx, m, n, k):
 # More than 64 rows of products too small for the tiles: 64 rows to a workgroup, the
 # last ones with 1 to 64, and depths shared by up to sixteen waves.
 MANY_SMALL = [(65, 33, 16), (65, 1300, 896), (100, 700, 272), (129, 2100, 1296), (191, 16, 640), (200, 1, 128),
-              (300, 130, 6848), (1000, 17, 400), (2049, 65, 144)]
+              (300, 130, 6848), (1000, 17, 400), (2049, 65, 144),
+              (129, 1900, 1296), (600, 500, 272)]
 
 
 @pytest.mark.parametrize("m,n,k", MANY_SMALL)
@@ -294,6 +295,21 @@ def test_linear_many_rows_of_small_products(ctx, m, n, k):
     say(f"small product {m}x{n}x{k}")
     test_linear_exact(ctx, m, n, k)
     test_linear_random(ctx, m, n, k)
+
+
+def test_linear_most_rows(ctx):
+    """As many rows as a call takes, of one column: whole numbers again."""
+    m, k = 1 << 22, 16
+    for rows in (m, m - 64, m - 65):
+        say(f"product {rows}x1x{k}")
+        x = (torch.arange(rows * k, device="cuda", dtype=torch.int64) % 9 - 4).float().view(rows, k)
+        w = torch.tensor([[float(i % 5) for i in range(k)]], device="cuda")
+        xq, wq = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
+        xs, ws = torch.full((rows, 1), 2.0, device="cuda"), torch.ones((1, 1), device="cuda")
+        y = torch.zeros((rows, 1), device="cuda")
+        torch.cuda.synchronize()
+        um.fp8_linear(ctx, xq, xs, wq, ws, y)
+        assert torch.equal(y[:, 0], 2 * (x * w).sum(1))
 
 
 def device_exact(m, n, k, seed):

@@ -315,7 +315,7 @@ def test_linear_logprobs_random(ctx, m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(65, 33, 16), (100, 700, 272), (129, 2100, 1296), (200, 1, 128),
-                                   (300, 130, 6848), (2049, 65, 144)])
+                                   (300, 130, 6848), (2049, 65, 144), (129, 1900, 1296), (600, 500, 272)])
 def test_linear_logprobs_many_rows_of_small_products(ctx, m, n, k):
     say(f"small fused scores {m}x{n}x{k}")
     test_linear_logprobs_exact_logits(ctx, m, n, k)
@@ -481,6 +481,62 @@ def test_other_heads(ctx, kind, T, V, H):
         extra = (H + 32 + H / 64 + 16) * U * float((np.abs(x) @ np.abs(w).T).max())
         compare(out.host(), reference(x @ w.T, tokens.cpu().numpy(), 0), extra)
     head.close()
+
+
+def fp8_head(ctx, norm, weight):
+    V, H = weight.shape
+    wq = torch.empty((V, H), dtype=torch.uint8, device="cuda")
+    ws = torch.empty((blocks(V), blocks(H)), device="cuda")
+    torch.cuda.synchronize()
+    um.fp8_quantize_weight(ctx, weight, wq, ws)
+    return um.LmHead(ctx, norm, 1e-6, q=wq, scales=ws, mode=um.QUANT_FP8_BLOCKS, where=um.MEMORY_DEVICE)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("H", [100, 1280, 2000, 2102])
+@pytest.mark.parametrize("top", [0, 3])
+def test_head_padding_rows_are_not_looked_at(ctx, kind, H, top):
+    """A padded batch: what lies in the padding rows (NaN, infinities) changes
+    nothing of the others and raises nothing."""
+    say(f"{kind} head with padding, H={H} top={top}")
+    rng = np.random.default_rng(H)
+    hidden, norm, weight, tokens = head_inputs(rng, 9, 700, H)
+    pad = [0, 4, 5, 8]
+    tokens[pad] = -1
+    head = fp8_head(ctx, norm, weight) if kind == "fp8" else \
+        um.LmHead(ctx, norm, 1e-6, weight=weight, where=um.MEMORY_DEVICE)
+    want, got = Scores(9, top), Scores(9, top)
+    torch.cuda.synchronize()
+    head.logprobs(ctx, hidden, tokens, **want.views())
+    hidden[0], hidden[4], hidden[5, 3], hidden[8, H - 1] = math.nan, math.inf, -math.inf, 3e38
+    torch.cuda.synchronize()
+    head.logprobs(ctx, hidden, tokens, **got.views())
+    a, b = want.host(), got.host()
+    for k in a:
+        assert np.array_equal(a[k], b[k]), k
+    assert (b["logprobs"][pad] == 0).all() and (b["entropy"][pad] == 0).all()
+    assert (b["logprobs"][[1, 2, 3, 6, 7]] < 0).all()
+    head.close()
+
+
+def test_head_of_many_logits_and_ragged_width():
+    """More outputs than one launch of the plain linear operator has waves for, in a
+    scratch that would hold them all: the rows are taken in turn."""
+    big = um.Context(0, 1 << 30)
+    T, V, H = 3500, 20000, 20
+    say(f"bf16 head T={T} V={V} H={H}")
+    hidden, norm, weight, tokens = head_inputs(np.random.default_rng(5), T, V, H)
+    head = um.LmHead(big, norm, 1e-6, weight=weight, where=um.MEMORY_DEVICE)
+    out = Scores(T, 0)
+    torch.cuda.synchronize()
+    head.logprobs(big, hidden, tokens, **out.views())
+    x, w = normalized(hidden, norm), weight.double().cpu().numpy()
+    rows = [0, 1, 1700, 3354, 3355, 3356, 3499]
+    extra = (H + 32 + H / 64 + 16) * U * float((np.abs(x[rows]) @ np.abs(w).T).max())
+    got = {k: v[rows] for k, v in out.host().items()}
+    compare(got, reference(x[rows] @ w.T, tokens.cpu().numpy()[rows], 0), extra)
+    head.close()
+    big.close()
 
 
 def test_head_refusals(ctx):

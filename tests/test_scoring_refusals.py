@@ -105,6 +105,7 @@ def test_head_logprobs():
 
 class FakeContext:
     handle = None
+    device = -1  # where host tensors are
 
 
 def refused(fn, *args, **kw):
@@ -144,3 +145,42 @@ def test_binding_checks_shapes():
                 (x, t, lp, lp, ids, tl[:, :3]), (x[0], t, lp)):
         assert refused(um.token_logprobs, *bad) == um.SHAPE
         assert "null context" not in message(um.token_logprobs, *bad)
+    # Types of the right size, and tensors that are somewhere else than the context.
+    e5m2 = torch.zeros(3, 200).to(torch.float8_e5m2)
+    assert refused(um.fp8_quantize, x, e5m2, s) == um.SHAPE
+    assert refused(um.fp8_quantize, x, q, s.int()) == um.SHAPE
+    assert refused(um.fp8_linear, e5m2, s, w, ws, y) == um.SHAPE
+    assert refused(um.fp8_linear, q, s, w, ws.int(), y) == um.SHAPE
+    assert refused(um.token_logprobs, x, t.float(), lp) == um.SHAPE
+    assert refused(um.token_logprobs, x, t, lp.int()) == um.SHAPE
+    assert refused(um.token_logprobs, x, t, lp, lp, tl, ids) == um.SHAPE
+    assert "null context" in message(um.fp8_linear_logprobs, q, s, w, ws, t, lp)
+
+    class OnGpu:
+        handle, device = None, 0
+    for fn, *args in ((um.fp8_quantize, x, q, s), (um.fp8_linear, q, s, w, ws, y),
+                      (um.token_logprobs, x, t, lp), (um.fp8_linear_logprobs, q, s, w, ws, t, lp)):
+        with pytest.raises(um.UocrError) as e:
+            fn(OnGpu, *args)
+        assert e.value.status == um.SHAPE and "device" in str(e.value)
+
+
+def test_head_binding():
+    class Head(um.LmHead):
+        def __init__(self):
+            self.handle, self.width = None, 64
+    hidden, t, lp = torch.zeros(3, 64), torch.zeros(3, dtype=torch.int32), torch.zeros(3)
+    head = Head()
+
+    def message(*args):
+        with pytest.raises(um.UocrError) as e:
+            head.logprobs(FakeContext, *args)
+        assert e.value.status == um.SHAPE
+        return str(e.value)
+    assert "null handle" in message(hidden, t, lp)
+    for bad in (hidden[:, :60], hidden.half(), hidden[0], torch.zeros(3, 128)[:, ::2], torch.zeros(3, 60)):
+        assert "null handle" not in message(bad, t, lp)
+    with pytest.raises(um.UocrError) as e:
+        um.LmHead(FakeContext, torch.ones(64), 1e-6, q=torch.zeros(300, 64, dtype=torch.uint8),
+                  scales=torch.ones(300, 2), mode=um.QUANT_FP8_BLOCKS)
+    assert e.value.status == um.SHAPE and "scales" in str(e.value)

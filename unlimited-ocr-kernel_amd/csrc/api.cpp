@@ -1321,6 +1321,14 @@ uocr::TokenScores scores_from(const uocr_token_scores& s, size_t row) {
   return o;
 }
 
+// Rows of one launch, which holds fewer than 2^32 threads: of a product with n
+// columns, and of a plain linear operator (a wave per output at ragged widths; at
+// others a workgroup takes kGemvChunk rows, in a dimension of at most 65535).
+size_t product_rows(size_t n) { return (((size_t)1 << 24) - 1) / fp8_blocks(n) * UOCR_FP8_BLOCK; }
+size_t linear_rows(size_t n, size_t k) {
+  return k % 64 == 0 ? (size_t)65535 * uocr::kGemvChunk : std::max<size_t>((((size_t)1 << 26) - 1) / n, 1);
+}
+
 // The most rows, at most m, whose need(rows) bytes fit (0: not even one).
 template <class Need>
 size_t rows_that_fit(size_t m, size_t limit, const Need& need) {
@@ -1494,6 +1502,7 @@ int uocr_lm_head_create(uocr_gpu_ctx* ctx, const uocr_lm_head_weights* w, uocr_m
   const bool fp8 = quant && w->quant_mode == UOCR_QUANT_FP8_BLOCKS;
   if (fp8) {
     if (!w->scales) return fail(UOCR_ERR_FORMAT, "missing lm_head.weight scales");
+    if (V > kMostRows || H > kMostCols) return fail(UOCR_ERR_RESOURCE, "too many rows or columns for one matrix");
   } else if (quant) {
     if (w->quant_mode != UOCR_QUANT_WEIGHTS_ONLY && w->quant_mode != UOCR_QUANT_DYNAMIC_ACTIVATIONS)
       return fail(UOCR_ERR_SHAPE, "an INT8 lm_head needs a quantization mode");
@@ -1576,18 +1585,20 @@ HeadRows head_rows(char* base, const uocr::LmHeadView& v, size_t rows) {
   return h;
 }
 
+// tokens: null, or the rows' tokens, negative ones for padding.
 void normalized_head_rows(uocr_gpu_ctx* ctx, const uocr::LmHeadView& v, const float* hidden,
-                          size_t rows, const HeadRows& h) {
+                          size_t rows, const HeadRows& h, const int32_t* tokens) {
   uocr::RowNorm nn;
   nn.w = v.norm_w;
   nn.eps = v.eps;
   nn.out = h.xn;
+  nn.tokens = tokens;
   uocr::launch_rms_norm(hidden, (int)rows, v.H, nn, ctx->err, ctx->stream);
 }
 
 void quantized_head_rows(uocr_gpu_ctx* ctx, const uocr::LmHeadView& v, const float* hidden,
-                         size_t rows, const HeadRows& h) {
-  normalized_head_rows(ctx, v, hidden, rows, h);
+                         size_t rows, const HeadRows& h, const int32_t* tokens) {
+  normalized_head_rows(ctx, v, hidden, rows, h, tokens);
   uocr::launch_fp8_quantize(h.xn, uocr::kTypeF32, rows, v.H, v.H, h.q, h.xs, ctx->err, ctx->stream);
 }
 
@@ -1611,7 +1622,7 @@ int uocr_lm_head_logits_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, const
   if (v.kind == 3) {
     const HeadRows rows = head_rows(ctx->scratch, v, 1);
     if (rows.bytes > ctx->scratch_limit) return scratch_fail(ctx);
-    quantized_head_rows(ctx, v, last, 1, rows);
+    quantized_head_rows(ctx, v, last, 1, rows, nullptr);
     uocr::launch_fp8_linear(fp8_head(v, rows, 1), logits, uocr::kTypeF32, nullptr, 0, ctx->stream);
   } else if (uocr::lm_head_fast(v.H)) {
     uocr::launch_lm_head(last, v, logits, ctx->err, ctx->stream);
@@ -1668,21 +1679,23 @@ int uocr_lm_head_logprobs_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, con
     return head_bytes + row8 + (fp8 ? product_need(fp8_head(v, {}, rows), rows, *scores)
                                     : logits_need(rows, V, *scores));
   };
-  const size_t step = std::min(rows_that_fit(T, ctx->scratch_limit, need),
-                               uocr::token_score_rows(v.V, uocr::kTypeF32));
+  const size_t step = std::min({rows_that_fit(T, ctx->scratch_limit, need),
+                                uocr::token_score_rows(v.V, uocr::kTypeF32),
+                                fp8 ? product_rows(V) : linear_rows(V, H)});
   if (!step) return scratch_fail(ctx);
   for (size_t t = 0; t < T; t += step) {
     const size_t rows = std::min(step, T - t);
     const float* in = hidden + t * H;
+    const int32_t* tokens = scores->tokens ? scores->tokens + t : nullptr;
     const HeadRows h = head_rows(ctx->scratch, v, rows);
     char* work = ctx->scratch + h.bytes;
     if (fp8) {
-      quantized_head_rows(ctx, v, in, rows, h);
+      quantized_head_rows(ctx, v, in, rows, h, tokens);
       enqueue_product_scores(ctx, fp8_head(v, h, rows), work, *scores, t);
     } else {
       float* logits = reinterpret_cast<float*>(work);
       char* after = work + align256(rows * V * 4);
-      normalized_head_rows(ctx, v, in, rows, h);
+      normalized_head_rows(ctx, v, in, rows, h, tokens);
       if (v.kind == 0) {
         uocr::launch_linear_bf16(h.xn, (int)rows, v.H, v.w, v.V, logits, ctx->stream);
       } else if (w8a8) {
@@ -1693,6 +1706,7 @@ int uocr_lm_head_logprobs_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, con
       } else {
         uocr::launch_int8_linear(v.q, v.s, v.V, v.H, h.xn, (int)rows, logits, ctx->stream);
       }
+      HIP_TRY(hipGetLastError(), "kernel launch");
       uocr::launch_token_scores(logits, uocr::kTypeF32, rows, v.V, V, scores_from(*scores, t), after,
                                 ctx->err, ctx->stream);
     }

@@ -217,9 +217,18 @@ void launch_combine(const Scratch& S, const float* residual, int T, int H, int K
 #undef UOCR_COMBINE
 }
 
+__device__ __forceinline__ bool is_padding(const RowNorm& nn, int t) { return nn.tokens && nn.tokens[t] < 0; }
+__device__ __forceinline__ void zero_row(float* out, int t, int width, int at, int step) {
+  for (int i = at; i < width; i += step) out[(size_t)t * width + i] = 0.0f;
+}
+
 __global__ __launch_bounds__(kRowThreads) void rms_norm_kernel(const float* __restrict__ x, int width,
                                                                RowNorm nn, int* err) {
   const int t = blockIdx.x;
+  if (is_padding(nn, t)) {
+    zero_row(nn.out, t, width, threadIdx.x, kRowThreads);
+    return;
+  }
   float4 row[kRowChunks];
 #pragma unroll
   for (int it = 0; it < kRowChunks; it++) {
@@ -238,6 +247,10 @@ __global__ __launch_bounds__(256) void rms_norm_wave_kernel(const float* __restr
   const int lane = threadIdx.x & 63;
   const int t = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
   if (t >= rows) return;
+  if (is_padding(nn, t)) {
+    zero_row(nn.out, t, width, lane, 64);
+    return;
+  }
   float4 row[kWaveChunks];
 #pragma unroll
   for (int it = 0; it < kWaveChunks; it++) {
@@ -251,11 +264,16 @@ __global__ __launch_bounds__(256) void rms_norm_wave_kernel(const float* __restr
 
 // Wider rows: one workgroup per row, scalar passes.
 __global__ __launch_bounds__(256) void rms_norm_wide_kernel(const float* __restrict__ x, int width,
-                                                            const float* __restrict__ w, float eps,
-                                                            float* __restrict__ out, int* err) {
+                                                            RowNorm nn, int* err) {
   __shared__ float partial[4];
   __shared__ int bad_any;
+  const float* __restrict__ w = nn.w;
+  float* __restrict__ out = nn.out;
   const int row = blockIdx.x;
+  if (is_padding(nn, row)) {
+    zero_row(out, row, width, threadIdx.x, 256);
+    return;
+  }
   const float* in = x + (size_t)row * width;
   if (threadIdx.x == 0) bad_any = 0;
   __syncthreads();
@@ -275,7 +293,7 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(const float* __restr
     if (threadIdx.x == 0) raise_error(err, kErrNumerical);
   }
   const float variance = total / (float)width;
-  const float scale = 1.0f / sqrtf(variance + eps);
+  const float scale = 1.0f / sqrtf(variance + nn.eps);
   for (int i = threadIdx.x; i < width; i += blockDim.x) out[(size_t)row * width + i] = in[i] * scale * w[i];
 }
 
@@ -290,7 +308,7 @@ void launch_rms_norm(const float* x, int rows, int width, const RowNorm& nn, int
   else if (row_norm_fusable(width))
     rms_norm_kernel<<<rows, kRowThreads, 0, s>>>(x, width, nn, err);
   else
-    rms_norm_wide_kernel<<<rows, 256, 0, s>>>(x, width, nn.w, nn.eps, nn.out, err);
+    rms_norm_wide_kernel<<<rows, 256, 0, s>>>(x, width, nn, err);
 }
 
 }  // namespace uocr

@@ -362,6 +362,7 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
 static bool takes_stream(const Fp8Product& p) {
   if (!whole_chunks(p)) return false;
   const size_t rows = (size_t)(p.m + kStreamRows - 1) / kStreamRows * kStreamRows;
+  if (rows / kStreamRows > 65535) return false;  // a grid's second dimension
   return p.m <= kStreamRows || rows * (size_t)p.n * p.kblocks() <= kStreamMost;
 }
 

@@ -293,13 +293,16 @@ void launch_rows_decode(const DeviceLayer& L, const Scratch& S, const float* res
 // combine.hip
 // RMSNorm output of rows: the normalised rows (out, [T, H]) and optionally
 // their bf16 planes (hi, and lo for FP32-class precision), k-blocked
-// ([H/32][T][32]) as the MFMA engine reads them.
+// ([H/32][T][32]) as the MFMA engine reads them. launch_rms_norm without planes
+// also takes `tokens` [T]: rows whose token is negative (padding) are not looked
+// at and come out as zeros.
 struct RowNorm {
   const float* w = nullptr;
   float eps = 0.0f;
   float* out = nullptr;
   uint16_t* hi = nullptr;
   uint16_t* lo = nullptr;
+  const int32_t* tokens = nullptr;
 };
 // Combine; with `next`, also the following layer's RMSNorm of the result.
 // y16: the expert outputs are bf16 rows (MFMA engine, BF16 activations).

@@ -419,6 +419,9 @@ class LmHead:
         self.handle = None
         src = weight if q is None else q
         V, H = src.shape
+        if q is not None and mode == QUANT_FP8_BLOCKS and scales is not None \
+                and tuple(scales.shape) != (-(-V // FP8_BLOCK), -(-H // FP8_BLOCK)):
+            _refuse("scales must be [ceil(V/128), ceil(H/128)]")
         keep = [norm_weight, weight, q, scales]
         w = LmHeadWeights(V, H, eps, _ptr(norm_weight), _ptr(weight), _ptr(q), _ptr(scales), mode)
         h = _P()
@@ -426,6 +429,7 @@ class LmHead:
         del keep
         self.handle = h
         self.vocab = V
+        self.width = H
 
     def logits(self, ctx: Context, hidden, out, sync: bool = True):
         fn = lib.uocr_lm_head_logits if sync else lib.uocr_lm_head_logits_async
@@ -434,8 +438,10 @@ class LmHead:
     def logprobs(self, ctx: Context, hidden, tokens=None, logprobs=None, entropy=None,
                  top_ids=None, top_logprobs=None, sync: bool = True):
         """Scores of the token after each row of hidden [T, H] (token_logprobs'
-        arguments)."""
-        s = _token_scores(hidden.shape[0], tokens, logprobs, entropy, top_ids, top_logprobs)
+        arguments); hidden is contiguous f32."""
+        if hidden.dim() != 2 or not _whole(hidden, (hidden.shape[0], self.width), 2, ctx.device):
+            _refuse("hidden must be contiguous f32 [T, H] on the context's device")
+        s = _token_scores(ctx, hidden.shape[0], tokens, logprobs, entropy, top_ids, top_logprobs)
         _check(_operator("uocr_lm_head_logprobs", sync)(ctx.handle, self.handle, _ptr(hidden),
                                                         hidden.shape[0], s))
 
@@ -508,43 +514,59 @@ def rms_norm(ctx: Context, x, weight, eps: float, out):
 FP8_BLOCK = 128
 MAX_TOP = 64
 
-# These checks stand between a tensor and its address, and cost a short call
-# more than its kernel: one condition per operand.
+# These checks stand between a tensor and its address (one on the host, or on another
+# GPU than the context's, would be read by a kernel), and cost a short call more than
+# its kernel: one condition per operand.
 
 
 def _refuse(message: str, status: int = SHAPE):
     raise UocrError(status, message)
 
 
-_types = {}
+_INT32, _FP8 = 32, 8  # beside the uocr_dtype codes of floating types
+
+
+class _Types(dict):
+    """torch dtype -> uocr_dtype, _INT32, _FP8 (e4m3, or its bytes) or -1."""
+
+    def __missing__(self, dtype):
+        code = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2, "torch.int32": _INT32,
+                "torch.float8_e4m3fn": _FP8, "torch.uint8": _FP8}.get(str(dtype), -1)
+        self[dtype] = code
+        return code
+
+
+_types = _Types()
 
 
 def _type(t) -> int:
     """uocr_dtype of a floating torch tensor (others: Unsupported)."""
-    code = _types.get(t.dtype)
-    if code is None:
-        code = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2}.get(str(t.dtype))
-        if code is None:
-            _refuse(f"element type {t.dtype}", UNSUPPORTED)
-        _types[t.dtype] = code
+    code = _types[t.dtype]
+    if not 0 <= code <= 2:
+        _refuse(f"element type {t.dtype}", UNSUPPORTED)
     return code
 
 
-def _rows(t, what: str):
+def _whole(t, shape, code: int, device: int) -> bool:
+    """Whether t is a contiguous tensor of that shape and type on the context's GPU."""
+    return t.shape == shape and _types[t.dtype] == code and t.is_contiguous() and t.get_device() == device
+
+
+def _rows(t, device: int, what: str):
     """(rows, columns, row stride) of a 2-D tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        _refuse(f"{what} must be rows")
+    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or t.get_device() != device:
+        _refuse(f"{what} must be rows on the context's device")
     rows, cols = t.shape
     return rows, cols, t.stride(0) if rows > 1 else max(cols, 1)
 
 
 def _quantize(fn, ctx, x, q, scales, tile: int):
-    rows, cols, ld = _rows(x, "x")
-    if q.shape != (rows, cols) or q.element_size() != 1 or not q.is_contiguous():
-        _refuse("q must be contiguous bytes of x's shape")
-    if scales.shape != (-(-rows // tile), -(-cols // 128)) or scales.element_size() != 4 \
-            or not scales.is_contiguous():
-        _refuse("scales must be one per block")
+    device = ctx.device
+    rows, cols, ld = _rows(x, device, "x")
+    if not _whole(q, (rows, cols), _FP8, device):
+        _refuse("q must be contiguous e4m3 bytes of x's shape, on the context's device")
+    if not _whole(scales, (-(-rows // tile), -(-cols // 128)), 2, device):
+        _refuse("scales must be f32, one per block, on the context's device")
     status = fn(ctx.handle, x.data_ptr(), _type(x), rows, cols, ld, q.data_ptr(),
                 scales.data_ptr())
     if status:
@@ -563,48 +585,53 @@ def fp8_quantize_weight(ctx: Context, w, q, scales):
     _quantize(_operator("uocr_fp8_quantize_weight"), ctx, w, q, scales, FP8_BLOCK)
 
 
-def _product(xq, xs, wq, ws):
+def _product(ctx, xq, xs, wq, ws):
     """The product's arguments (uocr_fp8_linear's second to eighth)."""
-    if xq.dim() != 2 or wq.dim() != 2 or xq.shape[1] != wq.shape[1]:
+    x, w = xq.shape, wq.shape
+    if len(x) != 2 or len(w) != 2 or x[1] != w[1]:
         _refuse("x [m, k] and w [n, k] must agree")
-    m, k = xq.shape
-    n = wq.shape[0]
-    blocks = -(-k // 128)
-    if xs.shape != (m, blocks) or ws.shape != (-(-n // 128), blocks):
+    m, k = x
+    n = w[0]
+    blocks = (k + 127) // 128
+    if xs.shape != (m, blocks) or ws.shape != ((n + 127) // 128, blocks):
         _refuse("scales must be [m, blocks(k)] and [blocks(n), blocks(k)]")
-    if not (xq.is_contiguous() and wq.is_contiguous() and xs.is_contiguous()
-            and ws.is_contiguous() and xq.element_size() == 1 and wq.element_size() == 1
-            and xs.element_size() == 4 and ws.element_size() == 4):
+    if not (_types[xq.dtype] == _types[wq.dtype] == _FP8 and _types[xs.dtype] == _types[ws.dtype] == 2
+            and xq.is_contiguous() and wq.is_contiguous() and xs.is_contiguous() and ws.is_contiguous()):
         _refuse("product operands must be contiguous e4m3 and f32")
+    if not xq.get_device() == wq.get_device() == xs.get_device() == ws.get_device() == ctx.device:
+        _refuse("product operands must be on the context's device")
     return xq.data_ptr(), xs.data_ptr(), m, k, wq.data_ptr(), ws.data_ptr(), n
 
 
 def fp8_linear(ctx: Context, xq, xs, wq, ws, y, sync: bool = True):
     """y [m, n] (f32 or bf16) = x . w^T of e4m3 rows xq [m, k] with scales xs and
     an e4m3 matrix wq [n, k] with scales ws per 128 x 128 tile."""
-    args = _product(xq, xs, wq, ws)
-    if y.shape != (args[2], args[6]) or not y.is_contiguous():
-        _refuse("y must be [m, n]")
+    args = _product(ctx, xq, xs, wq, ws)
+    if y.shape != (args[2], args[6]) or not y.is_contiguous() or y.get_device() != ctx.device:
+        _refuse("y must be [m, n] on the context's device")
     status = _operator("uocr_fp8_linear", sync)(ctx.handle, *args, y.data_ptr(), _type(y))
     if status:
         _check(status)
 
 
-def _score_address(t, shape):
+def _score_address(t, shape, code, device):
     if t is None:
         return None
-    if t.shape != shape or t.element_size() != 4 or not t.is_contiguous():
-        _refuse("score arrays must be contiguous 32-bit values, one per row (and alternative)")
+    if not _whole(t, shape, code, device):
+        _refuse("score arrays must be contiguous int32 ids and f32 scores, one per row (and "
+                "alternative), on the context's device")
     return t.data_ptr()
 
 
-def _token_scores(rows, tokens, logprobs, entropy, top_ids, top_logprobs) -> TokenScores:
+def _token_scores(ctx, rows, tokens, logprobs, entropy, top_ids, top_logprobs) -> TokenScores:
+    device = ctx.device
     one = (rows,)
     n_top = 0 if top_ids is None else top_ids.shape[-1]
     top = (rows, n_top)
-    return TokenScores(_score_address(tokens, one), n_top, _score_address(logprobs, one),
-                       _score_address(entropy, one), _score_address(top_ids, top),
-                       _score_address(top_logprobs, top))
+    return TokenScores(_score_address(tokens, one, _INT32, device), n_top,
+                       _score_address(logprobs, one, 2, device), _score_address(entropy, one, 2, device),
+                       _score_address(top_ids, top, _INT32, device),
+                       _score_address(top_logprobs, top, 2, device))
 
 
 def token_logprobs(ctx: Context, logits, tokens=None, logprobs=None, entropy=None, top_ids=None,
@@ -613,8 +640,8 @@ def token_logprobs(ctx: Context, logits, tokens=None, logprobs=None, entropy=Non
     probability of tokens [rows] (int32; negative: a padding row), the entropy,
     and the most probable ids top_ids [rows, n] (int32) with their log
     probabilities. Outputs are f32 tensors to fill; None skips one."""
-    rows, vocab, ld = _rows(logits, "logits")
-    s = _token_scores(rows, tokens, logprobs, entropy, top_ids, top_logprobs)
+    rows, vocab, ld = _rows(logits, ctx.device, "logits")
+    s = _token_scores(ctx, rows, tokens, logprobs, entropy, top_ids, top_logprobs)
     status = _operator("uocr_token_logprobs", sync)(ctx.handle, logits.data_ptr(), _type(logits),
                                                     rows, vocab, ld, s)
     if status:
@@ -625,8 +652,8 @@ def fp8_linear_logprobs(ctx: Context, xq, xs, wq, ws, tokens=None, logprobs=None
                         top_ids=None, top_logprobs=None, sync: bool = True):
     """token_logprobs of fp8_linear's product, without its logits in memory
     unless alternatives are asked for."""
-    args = _product(xq, xs, wq, ws)
-    s = _token_scores(args[2], tokens, logprobs, entropy, top_ids, top_logprobs)
+    args = _product(ctx, xq, xs, wq, ws)
+    s = _token_scores(ctx, args[2], tokens, logprobs, entropy, top_ids, top_logprobs)
     status = _operator("uocr_fp8_linear_logprobs", sync)(ctx.handle, *args, s)
     if status:
         _check(status)
