@@ -415,10 +415,9 @@ static void run_stream_rows(const Fp8Product& p, const ProductOut& out, int kind
 // waves, one per CU, hold x in LDS and stream the matrix with kWideDepth scale
 // blocks of 32 columns in flight per wave, across the ends of groups. Scores stay
 // in registers until the last group: one part per workgroup and row.
-// 129280 x 1280 (165 MB): one row 34 us (4.8 TB/s; the same loads alone take 28.5),
-// 48 rows 37 us, 64 rows 42 us. Four or five blocks in flight are slower (35 and 40
-// us for one and 48 rows), as are two workgroups per CU, and waves that load x from
-// the caches instead (39 and 66 us).
+// 129280 x 1280 (165 MB), scores: one row 33 us (5.0 TB/s; the same loads alone take
+// 28.5), 48 rows 38.6 us. Four or five blocks in flight are 2 to 3 us slower, as are two
+// workgroups per CU; waves that load x from the caches instead take 39 and 66 us.
 constexpr int kWideWaves = 8, kWideDepth = 2, kWideCols = 32;
 
 struct WideShape {
@@ -599,10 +598,14 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
     for (int j = 0; j < MB; j++)
       if (fg == 0) held[wave * (16 * MB) + 16 * j + fr] = sum[j];
     __syncthreads();
-    if (tid < 16 * MB && tid < p.m) {
-      ScorePart q = held[tid];
-      for (int w = 1; w < kWideWaves; w++) q = join(q, held[w * (16 * MB) + tid]);
-      out.parts[(size_t)blockIdx.x * p.m + tid] = q;
+    // Four threads to a row, two waves' parts each.
+    static_assert(kWideWaves == 8, "two parts to a thread");
+    const int row = tid / 4, w = 2 * (tid & 3);
+    if (row < 16 * MB) {
+      ScorePart q = join(held[w * (16 * MB) + row], held[(w + 1) * (16 * MB) + row]);
+      q = join(q, shfl_xor(q, 1));
+      q = join(q, shfl_xor(q, 2));
+      if ((tid & 3) == 0 && row < p.m) out.parts[(size_t)blockIdx.x * p.m + row] = q;
     }
   }
 }
@@ -679,8 +682,10 @@ size_t fp8_score_bytes(const Fp8Product& p) {
 // Joins the column tiles' statistics of each row. A workgroup of sixteen waves
 // takes R rows (1, 4, 16 or 64, the wave's lanes being R rows of 64 / R tiles each,
 // so that adjacent lanes read adjacent rows' parts): every thread some tiles, four
-// loads in flight, then the lanes and the waves of a row. With one row or some
-// dozens each thread has about one part: two dependent reads of memory in all.
+// loads in flight, then the lanes and the waves of a row, in trees. With one row or
+// some dozens each thread has about one part: two dependent reads of memory in all.
+// 256 parts of one row 4.8 us, of 48 rows 5.1 us, mostly the launch and those reads;
+// 1010 of 4096 rows 22 us.
 constexpr int kJoinWaves = 16;
 
 template <int R>
@@ -711,13 +716,20 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_parts_kernel(const Score
   for (int o = 32; o >= R; o >>= 1) p = join(p, shfl_xor(p, o));
   if (lane < R) held[wave][lane] = p;
   __syncthreads();
-  if (wave > 0 || lane >= R || row >= m) return;
+  if (wave > 0) return;
+  // The waves' parts likewise: 64 / R lanes to a row.
+  p = empty_part();
+#pragma unroll
+  for (int w = 0; w < kJoinWaves; w += 64 / R)
+    if (w + lane / R < kJoinWaves) p = join(p, held[w + lane / R][r]);
+#pragma unroll
+  for (int o = 32; o >= R; o >>= 1) p = join(p, shfl_xor(p, o));
+  if (lane >= R || row >= m) return;
   if (token < 0) {  // a padding row
     if (out.logprobs) out.logprobs[row] = 0.0f;
     if (out.entropy) out.entropy[row] = 0.0f;
     return;
   }
-  for (int w = 1; w < kJoinWaves; w++) p = join(p, held[w][r]);
   write_scores(out, row, token, vocab, p, logit, err);
 }
 
