@@ -712,8 +712,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_parts_kernel(const Score
       p = join(p, join(join(q[0], q[1]), join(q[2], q[3])));
     }
   }
-#pragma unroll
-  for (int o = 32; o >= R; o >>= 1) p = join(p, shfl_xor(p, o));
+  p = lanes_join<R>(p);
   if (lane < R) held[wave][lane] = p;
   __syncthreads();
   if (wave > 0) return;
@@ -722,8 +721,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_parts_kernel(const Score
 #pragma unroll
   for (int w = 0; w < kJoinWaves; w += 64 / R)
     if (w + lane / R < kJoinWaves) p = join(p, held[w + lane / R][r]);
-#pragma unroll
-  for (int o = 32; o >= R; o >>= 1) p = join(p, shfl_xor(p, o));
+  p = lanes_join<R>(p);
   if (lane >= R || row >= m) return;
   if (token < 0) {  // a padding row
     if (out.logprobs) out.logprobs[row] = 0.0f;

@@ -150,8 +150,9 @@ __global__ __launch_bounds__(kScoreThreads) void score_chunks_kernel(
       s[j & 1] += e;
       t[j & 1] = fmaf(e, fmaxf(d, -1000.0f), t[j & 1]);
     }
-  p.s = wave_sum(s[0] + s[1]);
-  p.t = wave_sum(t[0] + t[1]);
+  auto add = [](float a, float b) { return a + b; };
+  p.s = lanes_reduce<1>(s[0] + s[1], add);
+  p.t = lanes_reduce<1>(t[0] + t[1], add);
   if (lane == 0) parts[item] = p;
 }
 
@@ -176,7 +177,9 @@ constexpr int kMostGroups = 512, kMostCandidates = 1024;
 constexpr int kHeldMaxima = 8;
 
 // A chain of dependent reads (the maxima; then the candidates' logits) and barriers,
-// which is what it takes: everything that can be read early is.
+// which is what it takes: everything that can be read early is, and nothing that can
+// wait stands before a barrier. One row of 129280 f32 6.1 us: 1.7 to the maxima, 0.7 to
+// tau, 0.6 to the list, 1.2 to the candidates, 0.5 to the ranks.
 template <typename T>
 __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     const T* __restrict__ logits, int vocab, size_t ld, int chunks,
@@ -189,6 +192,8 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   __shared__ __attribute__((aligned(16))) float mine[kScoreThreads];
   __shared__ uint32_t tau_at;
   __shared__ int counts[2];
+  __shared__ float normalizer[2];
+  __shared__ bool good;
   const size_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int top = out.top;
@@ -212,7 +217,8 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     return;
   }
   const T* x = logits + row * ld;
-  const float given = tid == 0 && out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f;
+  constexpr int kScorer = kScoreThreads - 64;  // first thread of the last wave
+  const float given = tid == kScorer && out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f;
   // This thread's largest group.
   float most = g[0];
 #pragma unroll
@@ -226,8 +232,7 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   if (share >= 2) most = fmaxf(most, dpp_move<0xB1>(most));
   if (share == 4) most = fmaxf(most, dpp_move<0x4E>(most));
   if (tid % share == 0) mine[tid / share] = most;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) p = join(p, shfl_xor(p, o));
+  p = lanes_join<1>(p);
   if (lane == 0) held[wave] = p;
   if (tid < 2) counts[tid] = 0;
   if (tid == 0) tau_at = ~0u;
@@ -237,23 +242,33 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   if (top && tid < many) {
     const float v = mine[tid];
     int larger = 0;
+#pragma unroll 8
     for (int i = 0; i < many; i += 4) {
       const float4 o = *reinterpret_cast<const float4*>(mine + i);
       larger += (o.x > v) + (o.y > v) + (o.z > v) + (o.w > v);
     }
     if (larger < top) atomicMin(&tau_at, (uint32_t)(order_key(v, 0) >> 32));
   }
-  p = join(join(held[0], held[1]), join(held[2], held[3]));
-  if (tid == 0) write_scores(out, row, token, vocab, p, given, err);
+  // The last wave, which has no maximum to rank where four threads share one, joins
+  // the waves' statistics meanwhile.
+  if (tid >= kScorer) {
+    p = lanes_join<1>(lane < kScoreThreads / 64 ? held[lane] : empty_part());
+    if (lane == 0) {
+      write_scores(out, row, token, vocab, p, given, err);
+      good = has_distribution(p);
+      normalizer[0] = p.r;
+      normalizer[1] = kLn2 * log2f(p.s);
+    }
+  }
   if (top == 0) return;
-  if (!has_distribution(p)) {
+  __syncthreads();
+  if (!good) {
     for (int i = tid; i < top; i += kScoreThreads) {
       out.top_ids[row * top + i] = -1;
       out.top_logprobs[row * top + i] = __uint_as_float(0x7fc00000u);
     }
     return;
   }
-  __syncthreads();
   const float tau = key_value((unsigned long long)tau_at << 32);
   // With tau -inf (fewer finite logits than alternatives, or nearly): all finite
   // logits, and the first columns' banned ones to fill up with.
@@ -290,10 +305,9 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     }
     __syncthreads();
   }
-  const float l = kLn2 * log2f(p.s);
   auto write = [&](int at, unsigned long long key) {
     out.top_ids[row * top + at] = (int32_t)key_index(key);
-    out.top_logprobs[row * top + at] = key_value(key) - p.r - l;
+    out.top_logprobs[row * top + at] = key_value(key) - normalizer[0] - normalizer[1];
   };
   const int found = counts[1];
   if (some <= kMostGroups && found <= kMostCandidates) {

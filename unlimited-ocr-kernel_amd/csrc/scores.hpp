@@ -53,6 +53,33 @@ __device__ __forceinline__ ScorePart shfl_xor(const ScorePart& p, int o) {
   return {__shfl_xor(p.r, o), __shfl_xor(p.s, o), __shfl_xor(p.t, o), 0.0f};
 }
 
+// op over the lanes of equal lane % R (a power of two), in each of them: rotations
+// within rows of 16 lanes, then across the rows.
+template <int R, class Op>
+__device__ __forceinline__ float lanes_reduce(float v, const Op& op) {
+  if (R <= 1) v = op(v, dpp_move<0x121>(v));
+  if (R <= 2) v = op(v, dpp_move<0x122>(v));
+  if (R <= 4) v = op(v, dpp_move<0x124>(v));
+  if (R <= 8) v = op(v, dpp_move<0x128>(v));
+  if (R <= 16) v = op(v, __shfl_xor(v, 16));
+  if (R <= 32) v = op(v, __shfl_xor(v, 32));
+  return v;
+}
+// The join of those lanes' parts, all moved to their largest reference at once: one
+// exponential instead of two for each pair.
+template <int R>
+__device__ __forceinline__ ScorePart lanes_join(const ScorePart& p) {
+  const bool some = p.s != 0.0f;  // a NaN counts
+  auto add = [](float a, float b) { return a + b; };
+  ScorePart o;
+  o.r = lanes_reduce<R>(some ? p.r : -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+  const float d = (p.r - o.r) * kLog2e, e = __builtin_amdgcn_exp2f(d);
+  o.s = lanes_reduce<R>(some ? p.s * e : 0.0f, add);
+  o.t = lanes_reduce<R>(some && e != 0.0f ? e * fmaf(p.s, d, p.t) : 0.0f, add);
+  o.unused = 0.0f;
+  return o;
+}
+
 // A key that orders logits by value descending, then by index ascending, as
 // unsigned numbers; -0 equals 0.
 __device__ __forceinline__ unsigned long long order_key(float v, uint32_t index) {
