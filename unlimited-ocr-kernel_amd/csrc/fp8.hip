@@ -196,12 +196,8 @@ void launch_fp8_quantize_tiles(const void* x, int type, int rows, int cols, size
 // workgroup share a group's depth and add up in LDS, in order. Lane l reads the bytes
 // [16 (l / 16), +16) and 64 bytes on of row l % 16 in each block: a load instruction
 // covers 64-byte runs.
-// More than 64 rows stay here while rows (whole 64) x columns x scale blocks are at
-// most kStreamMost, where the tiles' fewer workgroups leave most of the card idle.
-// Time on tiles over time here, bf16 / f32 results: at 1 to 2 Mi 1.1 to 2.1; at 4 Mi
-// 0.86 / 1.18 (512 x 1280 x 896), 1.27 / 1.85 (512 x 896 x 1280), 1.17 / 1.31 (128 x
-// 2560 x 1792); at 8 Mi 0.62 to 0.77 / 0.85 to 1.11; beyond 16 Mi the tiles win.
 constexpr int kStreamRows = 64;
+// More than 64 rows come here only up to this many rows (whole 64) x columns x blocks.
 constexpr size_t kStreamMost = (size_t)4 << 20;
 
 struct StreamShape {
@@ -359,13 +355,6 @@ __global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kerne
   }
 }
 
-static bool takes_stream(const Fp8Product& p) {
-  if (!whole_chunks(p)) return false;
-  const size_t rows = (size_t)(p.m + kStreamRows - 1) / kStreamRows * kStreamRows;
-  if (rows / kStreamRows > 65535) return false;  // a grid's second dimension
-  return p.m <= kStreamRows || rows * (size_t)p.n * p.kblocks() <= kStreamMost;
-}
-
 struct StreamPlan {
   int rg, mb;
   StreamShape shape;
@@ -391,6 +380,24 @@ static StreamPlan plan_stream(const Fp8Product& p, bool scores) {
   s.lds = ks > 1 ? (size_t)s.shape.waves * s.rg * s.mb * 64 * sizeof(f32x4) : 0;
   if (scores) s.lds = std::max(s.lds, (size_t)per * 16 * s.mb * sizeof(ScorePart));
   return s;
+}
+
+// Few rows, or a small product, where the tiles would leave most of the card idle: by a
+// model of both times. A CU's loads set the time here, 25 bytes per ns of x and of the
+// matrix; measured against the model 0.75 to 1.2. f32 results here and on tiles: 16 x
+// 6848 x 1280 5.7 and 8.3 us, 64 x 1280 x 1280 7.1 and 7.5, 48 x 4096 x 4096 13.8 and
+// 12.8, 64 x 1280 x 6848 19.5 and 12.7, 512 x 896 x 1280 8.7 and 11.2, 512 x 1280 x 896
+// 10.4 and 8.9, 1 x 20000 x 1280 8.8 and 10.7, 32 x 20000 x 1280 16.2 and 11.5.
+static bool takes_stream(const Fp8Product& p, int kind, size_t work_bytes) {
+  if (!whole_chunks(p)) return false;
+  const size_t rows = (size_t)(p.m + kStreamRows - 1) / kStreamRows * kStreamRows;
+  if (rows / kStreamRows > 65535) return false;  // a grid's second dimension
+  if (p.m > kStreamRows && rows * (size_t)p.n * p.kblocks() > kStreamMost) return false;
+  const StreamPlan t = plan_stream(p, kind == kOutScores);
+  const size_t rounds = ((size_t)t.grid.x * t.grid.y + kCus - 1) / kCus;
+  const size_t bytes =
+      rounds * (t.shape.waves / t.shape.ks) * (16 * t.rg + std::min(p.m, kStreamRows)) * (size_t)p.k;
+  return 26 + bytes * 4e-4 <= fp8_gemm_time(p, kind != kOutBf16, work_bytes);
 }
 
 template <int MB, int RG>
@@ -651,7 +658,7 @@ static void launch_product(const Fp8Product& p, const ProductOut& out, int kind,
     if (mb == 2) run_wide<2>(p, out, kind, s);
     if (mb == 3) run_wide<3>(p, out, kind, s);
     if (mb == 4) run_wide<4>(p, out, kind, s);
-  } else if (takes_stream(p)) {
+  } else if (takes_stream(p, kind, work_bytes)) {
     const StreamPlan t = plan_stream(p, kind == kOutScores);
     t.rg == 2 ? run_stream_rows<2>(p, out, kind, t, s) : run_stream_rows<1>(p, out, kind, t, s);
   } else {
@@ -667,8 +674,8 @@ void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, void* work, size
 
 // Parts per row.
 static int score_tiles(const Fp8Product& p) {
-  if (!takes_stream(p)) return fp8_gemm_parts(p);
-  return takes_wide(p) ? kCus : (int)plan_stream(p, true).grid.x;
+  if (takes_wide(p)) return kCus;
+  return takes_stream(p, kOutScores, 0) ? (int)plan_stream(p, true).grid.x : fp8_gemm_parts(p);
 }
 
 size_t fp8_score_bytes(const Fp8Product& p) {

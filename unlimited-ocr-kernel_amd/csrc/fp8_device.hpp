@@ -125,6 +125,8 @@ int fp8_gemm_parts(const Fp8Product& p);
 void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
                      hipStream_t s);
 void fp8_gemm_init_attributes();
+// The launch's modelled time in units of 0.1 us (whole_chunks only).
+double fp8_gemm_time(const Fp8Product& p, bool widen, size_t work_bytes);
 
 // Whole 16-byte chunks of rows at aligned addresses.
 inline bool whole_chunks(const Fp8Product& p) {

@@ -104,9 +104,10 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 }
 
 // ---- whole 16-byte chunks: 128 x 128 outputs per workgroup of four waves, 64 x 64
-// each. A stage is one scale block deep: 256 rows of 128 bytes, brought by global->LDS
-// loads into a ring of buffers ahead of the one that is multiplied. The matrix is the matrix instruction's first operand: lane l then holds four adjacent
-// columns of y for row l % 16, whose x scale it needs as one value.
+// each, or 64 x 128 and 32 x 64. A stage is one scale block deep: 256 rows of 128 bytes, brought by global->LDS
+// loads into a ring of buffers ahead of the one that is multiplied. The matrix is the matrix
+// instruction's first operand: lane l then holds four adjacent columns of y for row
+// l % 16, whose x scale it needs as one value.
 //
 // WIDEN: the matrix cores' e4m3 instructions bring each group of eight products to
 // the largest one's exponent and cut them off 13 bits below it (measured: 2^16 -
@@ -117,16 +118,24 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 // per scale block, at twice the rate. Either way a block's sum is scaled into the f32
 // accumulators when it is done.
 //
-// BUFS stages of LDS: with two, two workgroups share a CU and hide each other's waits
-// (many tiles); with four, one workgroup keeps three stages in flight (few tiles, where
-// the wait for memory is what counts). Few tiles of a long depth are also split along
-// it: each split leaves f32 partial sums in memory, and a second launch adds them in
-// order.
-constexpr int kTile = 128, kXb = 4;  // rows and columns of a tile, row blocks of a wave
-constexpr uint32_t kStage = 2 * kTile * 128u;
-// Scales of eight blocks: x's [8][kTile], the matrix's [8].
-constexpr uint32_t kScales = (8 * kTile + 8) * 4u;
-constexpr size_t tile_lds(int bufs) { return bufs * kStage + 2 * kScales; }
+// BUFS stages of LDS, so that two workgroups share a CU and hide each other's waits: two
+// stages with tiles of 128 rows, three with tiles of 64. Where there are no more tiles of
+// 128 than CUs, those of 64 are taken: more of them, less padding, and a stage more in
+// flight (277 x 1280 x 6848 f32 20.9 -> 17.3 us, 1024 x 1280 x 896 bf16 9.6 -> 7.1; beyond,
+// 1024 x 6848 x 1280 bf16 is 18.4 us with 128 rows and 21.8 with 64). Few tiles of a long
+// depth are also split along it: each split leaves f32 partial sums in memory, and a
+// second launch adds them in order.
+//
+// 4096 x 6848 x 1280 bf16 55 us (1310 TFLOP/s): the loads bring 17 TB/s into LDS, which is
+// what bounds the steps, and the stores take 10 us. 4096 x 129280 x 1280 scores 1275 us
+// (1060 TFLOP/s): the vector instructions, 3.4 a product (2 of widening, 1 of scaling) and
+// the statistics', share the issue with the products.
+constexpr int kCols = 128;  // columns of a tile
+constexpr int tile_rows(int xb) { return 32 * xb; }  // for xb blocks of 16 rows in each of two waves
+constexpr uint32_t stage_bytes(int xb) { return (tile_rows(xb) + kCols) * 128u; }
+// Scales of eight blocks: x's [8][rows of the tile], the matrix's [8].
+constexpr uint32_t scale_bytes(int xb) { return (8 * tile_rows(xb) + 8) * 4u; }
+constexpr size_t tile_lds(int bufs, int xb) { return bufs * stage_bytes(xb) + 2 * scale_bytes(xb); }
 
 // Workgroups reach the 8 XCDs round-robin, each XCD with an L2 of its own. They are
 // renumbered so that an XCD takes a contiguous run of tiles, and tiles run down strips
@@ -150,45 +159,48 @@ struct Splits {
   int count, each;
 };
 
-template <bool WIDEN, int OUT, int BUFS>
+template <bool WIDEN, int OUT, int BUFS, int XB>
 __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductOut out, Splits splits) {
-  constexpr int XB = kXb;
+  constexpr int kRows = tile_rows(XB);
+  constexpr uint32_t kStage = stage_bytes(XB), kScales = scale_bytes(XB);
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, fg = lane >> 4;
   const int K = p.k, nkb = p.kblocks();
-  const int tiles_m = (p.m + kTile - 1) / kTile, tiles_n = (p.n + kTile - 1) / kTile;
+  const int tiles_m = (p.m + kRows - 1) / kRows, tiles_n = (p.n + kCols - 1) / kCols;
   // The splits of a tile lie far apart: an XCD works on neighbouring tiles at one depth.
   const int split = (int)blockIdx.x / (tiles_m * tiles_n);
   const TileAt tile = tile_of((int)blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n);
   const int first = split * splits.each, last = min(nkb, first + splits.each);
-  const int m0 = tile.m * kTile, n0 = tile.n * kTile;
-  const int wm = wave / 2 * 64, wn = wave % 2 * 64;
+  const int m0 = tile.m * kRows, n0 = tile.n * kCols;
+  const int wm = wave / 2 * (16 * XB), wn = wave % 2 * 64;
 
   // Loads: a wave instruction brings 8 rows of 128 bytes; chunk c of row r lies at c
   // ^ (r % 8), which spreads a fragment read's sixteen rows over all banks.
-  constexpr int kSegs = kTile / 8 / 4, kLoads = 2 * kSegs;
-  const i32x4 rx = buffer_rsrc(p.x + (size_t)m0 * K, (uint32_t)min(kTile, p.m - m0) * K);
-  const i32x4 rw = buffer_rsrc(p.w + (size_t)n0 * K, (uint32_t)min(kTile, p.n - n0) * K);
+  constexpr int kSegsX = kRows / 8 / 4, kSegsW = kCols / 8 / 4, kLoads = kSegsX + kSegsW;
+  const i32x4 rx = buffer_rsrc(p.x + (size_t)m0 * K, (uint32_t)min(kRows, p.m - m0) * K);
+  const i32x4 rw = buffer_rsrc(p.w + (size_t)n0 * K, (uint32_t)min(kCols, p.n - n0) * K);
   const int chunk = (lane & 7) ^ (lane >> 3);
-  const uint32_t at = (uint32_t)(wave * kSegs * 8 + (lane >> 3)) * K + 16 * chunk;
+  const uint32_t at_x = (uint32_t)(wave * kSegsX * 8 + (lane >> 3)) * K + 16 * chunk;
+  const uint32_t at_w = (uint32_t)(wave * kSegsW * 8 + (lane >> 3)) * K + 16 * chunk;
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
   auto issue = [&](int kb) {
     const uint32_t k = (uint32_t)kb * 128u;
     const uint32_t past = (int)k + 16 * chunk < K ? 0u : kDmaOut;
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(kb % BUFS) * kStage);
 #pragma unroll
-    for (int i = 0; i < kSegs; i++) {
-      const uint32_t off = (at + (uint32_t)(8 * i) * K + k) | past;
-      buffer_load_lds16(rx, to + (uint32_t)(wave * kSegs + i) * 1024u, off);
-      buffer_load_lds16(rw, to + kTile * 128u + (uint32_t)(wave * kSegs + i) * 1024u, off);
+    for (int i = 0; i < kSegsW; i++) {
+      if (i < kSegsX)
+        buffer_load_lds16(rx, to + (uint32_t)(wave * kSegsX + i) * 1024u, (at_x + (uint32_t)(8 * i) * K + k) | past);
+      buffer_load_lds16(rw, to + kRows * 128u + (uint32_t)(wave * kSegsW + i) * 1024u,
+                        (at_w + (uint32_t)(8 * i) * K + k) | past);
     }
   };
   // Scales of eight blocks at a time, in LDS beside the stages. A thread brings four
   // blocks of one row of x (16 bytes; a lane per row and block, 4 bytes each of a line
   // of its own, took as long as the stages), some one of the matrix's.
-  const __amdgpu_buffer_rsrc_t rxs = read_rsrc(p.xs + (size_t)m0 * nkb, (uint32_t)(min(kTile, p.m - m0) * nkb) * 4u);
+  const __amdgpu_buffer_rsrc_t rxs = read_rsrc(p.xs + (size_t)m0 * nkb, (uint32_t)(min(kRows, p.m - m0) * nkb) * 4u);
   const __amdgpu_buffer_rsrc_t rws = read_rsrc(p.ws + (size_t)tile.n * nkb, (uint32_t)nkb * 4u);
   struct Scales {
     u32x4 x;
@@ -203,9 +215,10 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
   auto scales_at = [&](int eighth) { return reinterpret_cast<float*>(lds + BUFS * kStage + (eighth & 1) * kScales); };
   auto store_scales = [&](int eighth, const Scales& s) {
     float* to = scales_at(eighth);
+    if (kRows == 128 || tid < 2 * kRows)
 #pragma unroll
-    for (int i = 0; i < 4; i++) to[(4 * (tid & 1) + i) * kTile + (tid >> 1)] = __uint_as_float(s.x[i]);
-    if (tid < 8) to[8 * kTile + tid] = __uint_as_float(s.w);
+      for (int i = 0; i < 4; i++) to[(4 * (tid & 1) + i) * kRows + (tid >> 1)] = __uint_as_float(s.x[i]);
+    if (tid < 8) to[8 * kRows + tid] = __uint_as_float(s.w);
   };
 
   f32x4 acc[4][XB];
@@ -233,9 +246,9 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
   };
   auto multiply = [&](int kb) {
     const char* xt = lds + (size_t)(kb % BUFS) * kStage;
-    const char* wt = xt + kTile * 128;
-    const float* xs = scales_at(kb >> 3) + (kb & 7) * kTile + wm + fr;
-    const float ws = scales_at(kb >> 3)[8 * kTile + (kb & 7)];
+    const char* wt = xt + kRows * 128;
+    const float* xs = scales_at(kb >> 3) + (kb & 7) * kRows + wm + fr;
+    const float ws = scales_at(kb >> 3)[8 * kRows + (kb & 7)];
     float sc[2];
     f32x4 d[2][4];
     auto zero = [&](f32x4 (&v)[4]) {
@@ -339,11 +352,11 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
       const f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
       ScorePart q = empty_part();
       if (n0 + wn < p.n) q = row_statistics<4>(v, n0 + wn, fg, p.n, token, out.given + row);
-      if (fg == 0) held[wave % 2 * kTile + r] = q;
+      if (fg == 0) held[wave % 2 * kRows + r] = q;
     }
     __syncthreads();
-    if (tid < kTile && m0 + tid < p.m)
-      out.parts[(size_t)tile.n * p.m + m0 + tid] = join(held[tid], held[kTile + tid]);
+    if (tid < kRows && m0 + tid < p.m)
+      out.parts[(size_t)tile.n * p.m + m0 + tid] = join(held[tid], held[kRows + tid]);
   } else {
     char* y = static_cast<char*>(out.y) + (size_t)split * p.m * p.n * (OUT == kOutF32 ? 4 : 2);
 #pragma unroll
@@ -388,49 +401,78 @@ __global__ __launch_bounds__(256) void add_splits_kernel(const float* __restrict
   }
 }
 
-template <bool WIDEN, int OUT, int BUFS>
+static size_t tiles_of(const Fp8Product& p, int rows) {
+  return (size_t)((p.n + kCols - 1) / kCols) * ((p.m + rows - 1) / rows);
+}
+
+template <bool WIDEN, int OUT, int BUFS, int XB>
 static void run_tiles(const Fp8Product& p, const ProductOut& out, const Splits& splits, hipStream_t s) {
-  const unsigned tiles = (unsigned)((p.n + kTile - 1) / kTile) * (unsigned)((p.m + kTile - 1) / kTile);
-  fp8_tile_kernel<WIDEN, OUT, BUFS><<<tiles * splits.count, 256, tile_lds(BUFS), s>>>(p, out, splits);
+  fp8_tile_kernel<WIDEN, OUT, BUFS, XB>
+      <<<(unsigned)(tiles_of(p, tile_rows(XB)) * splits.count), 256, tile_lds(BUFS, XB), s>>>(p, out, splits);
+}
+// Tiles of 128 rows, or (more of them, with less padding) of 64.
+template <bool WIDEN, int OUT>
+static void run_tall(const Fp8Product& p, const ProductOut& out, hipStream_t s) {
+  run_tiles<WIDEN, OUT, 2, 4>(p, out, {1, p.kblocks()}, s);
+}
+template <bool WIDEN, int OUT>
+static void run_short(const Fp8Product& p, const ProductOut& out, const Splits& splits, hipStream_t s) {
+  run_tiles<WIDEN, OUT, 3, 2>(p, out, splits, s);
 }
 
-// Two workgroups per CU need twice as many tiles as there are CUs.
-static bool many_tiles(const Fp8Product& p) {
-  return (size_t)((p.n + kTile - 1) / kTile) * ((p.m + kTile - 1) / kTile) > (size_t)kCus;
+static bool takes_tall(const Fp8Product& p) { return tiles_of(p, tile_rows(4)) > (size_t)kCus; }
+
+// A model of the time in units of 0.1 us, with what was measured for its parts: a
+// workgroup's start and end 35; a step of one that has a CU to itself 7.7 (WIDEN) or 4.5,
+// of two that share one 12 or 7; with tall tiles twice that.
+static double tiles_time(size_t workgroups, int steps, bool widen, bool tall) {
+  const double size = tall ? 2.0 : 1.0, alone = size * (widen ? 7.7 : 4.5), shared = size * (widen ? 12.0 : 7.0);
+  const size_t full = workgroups / (2 * kCus), rest = workgroups % (2 * kCus);
+  return full * (35 + shared * steps) + (rest ? 35 + (rest > (size_t)kCus ? shared : alone) * steps : 0.0);
 }
 
-// How many ways to split the depth: by a model of the time in units of 0.1 us, with what
-// was measured for its parts: a step of a workgroup that has a CU to itself 6, a round of
-// workgroups' start and end 30, the second launch 25 and its traffic 5 GB/ms each way.
-static Splits plan_splits(const Fp8Product& p, size_t work_bytes) {
+// How many ways to split the depth, and the modelled time: the second launch takes 30 and
+// its traffic 5 GB/ms each way. Of 1 to 10 ways this takes the best or one within 3%.
+constexpr int kMostSplits = 64;
+struct TilePlan {
+  Splits splits;
+  double time;
+};
+static TilePlan plan_splits(const Fp8Product& p, bool widen, size_t work_bytes) {
   const int nkb = p.kblocks();
-  Splits best{1, nkb};
-  if (many_tiles(p)) return best;
-  const size_t tiles = (size_t)((p.n + kTile - 1) / kTile) * ((p.m + kTile - 1) / kTile), bytes = (size_t)p.m * p.n * 4;
-  double least = 1e30;
-  for (int each = nkb; each >= 2; each--) {
-    const int count = (nkb + each - 1) / each;
-    if (count > 1 && count * bytes > work_bytes) break;
-    const double rounds = (double)((tiles * count + kCus - 1) / kCus);
-    const double time = rounds * (30 + 6.0 * each) + (count > 1 ? 25 + 2.0 * count * bytes / 5e5 : 0.0);
-    if (time < least) {
-      least = time;
-      best = {count, each};
-    }
+  const size_t tiles = tiles_of(p, tile_rows(2)), bytes = (size_t)p.m * p.n * 4;
+  TilePlan best{{1, nkb}, tiles_time(tiles, nkb, widen, false)};
+  for (int ways = 2; ways <= std::min(kMostSplits, nkb / 2); ways++) {
+    const int each = (nkb + ways - 1) / ways, count = (nkb + each - 1) / each;
+    if (count * bytes > work_bytes) break;
+    const double time = tiles_time(tiles * count, each, widen, false) + 30 + 2.0 * count * bytes / 5e5;
+    if (time < best.time) best = {{count, each}, time};
   }
   return best;
 }
 
-int fp8_gemm_parts(const Fp8Product& p) {
-  return whole_chunks(p) ? (p.n + kTile - 1) / kTile : (p.n + 63) / 64;
+double fp8_gemm_time(const Fp8Product& p, bool widen, size_t work_bytes) {
+  return takes_tall(p) ? tiles_time(tiles_of(p, tile_rows(4)), p.kblocks(), widen, true)
+                       : plan_splits(p, widen, work_bytes).time;
 }
 
+int fp8_gemm_parts(const Fp8Product& p) {
+  return whole_chunks(p) ? (p.n + kCols - 1) / kCols : (p.n + 63) / 64;
+}
+
+template <bool WIDEN, int OUT, int BUFS, int XB>
+static void tile_attributes() {
+  (void)hipFuncSetAttribute((const void*)fp8_tile_kernel<WIDEN, OUT, BUFS, XB>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
+}
 void fp8_gemm_init_attributes() {
-  const void* kernels[] = {(const void*)fp8_tile_kernel<false, kOutBf16, 2>, (const void*)fp8_tile_kernel<false, kOutBf16, 4>,
-                           (const void*)fp8_tile_kernel<false, kOutF32, 4>, (const void*)fp8_tile_kernel<true, kOutF32, 2>,
-                           (const void*)fp8_tile_kernel<true, kOutF32, 4>, (const void*)fp8_tile_kernel<true, kOutScores, 2>,
-                           (const void*)fp8_tile_kernel<true, kOutScores, 4>};
-  for (const void* k : kernels) (void)hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
+  tile_attributes<false, kOutBf16, 2, 4>();
+  tile_attributes<true, kOutF32, 2, 4>();
+  tile_attributes<true, kOutScores, 2, 4>();
+  tile_attributes<false, kOutBf16, 3, 2>();
+  tile_attributes<false, kOutF32, 3, 2>();
+  tile_attributes<true, kOutF32, 3, 2>();
+  tile_attributes<true, kOutScores, 3, 2>();
 }
 
 void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
@@ -445,28 +487,32 @@ void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, void*
       fp8_bytes_kernel<kOutScores><<<grid, 256, 0, s>>>(p, out);
     return;
   }
-  const bool many = many_tiles(p);
-  const Splits one{1, p.kblocks()};
-  if (kind == kOutScores) {
-    many ? run_tiles<true, kOutScores, 2>(p, out, one, s) : run_tiles<true, kOutScores, 4>(p, out, one, s);
+  if (takes_tall(p)) {
+    if (kind == kOutF32)
+      run_tall<true, kOutF32>(p, out, s);
+    else if (kind == kOutBf16)
+      run_tall<false, kOutBf16>(p, out, s);
+    else
+      run_tall<true, kOutScores>(p, out, s);
     return;
   }
-  const Splits splits = plan_splits(p, work_bytes);
+  if (kind == kOutScores) {
+    run_short<true, kOutScores>(p, out, {1, p.kblocks()}, s);
+    return;
+  }
+  const Splits splits = plan_splits(p, kind == kOutF32, work_bytes).splits;
   if (splits.count == 1) {
-    if (kind == kOutF32)
-      many ? run_tiles<true, kOutF32, 2>(p, out, one, s) : run_tiles<true, kOutF32, 4>(p, out, one, s);
-    else
-      many ? run_tiles<false, kOutBf16, 2>(p, out, one, s) : run_tiles<false, kOutBf16, 4>(p, out, one, s);
+    kind == kOutF32 ? run_short<true, kOutF32>(p, out, splits, s) : run_short<false, kOutBf16>(p, out, splits, s);
     return;
   }
   const ProductOut parts{work, nullptr, nullptr, nullptr};
   const size_t count = (size_t)p.m * p.n;
   const unsigned grid = (unsigned)((count + 1023) / 1024);
   if (kind == kOutF32) {
-    run_tiles<true, kOutF32, 4>(p, parts, splits, s);
+    run_short<true, kOutF32>(p, parts, splits, s);
     add_splits_kernel<kOutF32><<<grid, 256, 0, s>>>((const float*)work, count, splits.count, out.y);
   } else {
-    run_tiles<false, kOutF32, 4>(p, parts, splits, s);
+    run_short<false, kOutF32>(p, parts, splits, s);
     add_splits_kernel<kOutBf16><<<grid, 256, 0, s>>>((const float*)work, count, splits.count, out.y);
   }
 }
