@@ -207,11 +207,11 @@ struct StreamShape {
 // Blocks in flight.
 constexpr int kStreamDepth = 2;
 // Most waves of a workgroup, by the registers that a wave then may have: 128 where
-// x has one or two blocks of rows and a wave one group of columns, 256 otherwise.
-constexpr int stream_waves(int mb, int rg) { return rg == 1 && mb <= 2 ? 16 : 8; }
+// x has one or two blocks of rows, 256 otherwise.
+constexpr int stream_waves(int mb) { return mb <= 2 ? 16 : 8; }
 
 template <int MB, int RG, int OUT>
-__global__ __launch_bounds__(64 * stream_waves(MB, RG), 2) void fp8_stream_kernel(Fp8Product p, ProductOut out,
+__global__ __launch_bounds__(64 * stream_waves(MB), 2) void fp8_stream_kernel(Fp8Product p, ProductOut out,
                                                                                   StreamShape shape) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -365,11 +365,13 @@ static StreamPlan plan_stream(const Fp8Product& p, bool scores) {
   StreamPlan s;
   const int chunks = (p.m + kStreamRows - 1) / kStreamRows;
   s.mb = (std::min(p.m, kStreamRows) + 15) / 16;
-  s.rg = (p.n + 31) / 32 * chunks >= (chunks > 1 ? 128 : 2048) ? 2 : 1;
+  // Two groups of columns to a wave, which reads x half as often, where whole 64 rows are
+  // enough work for half of the CUs all the same.
+  s.rg = chunks > 1 && (p.n + 31) / 32 * chunks >= 128 ? 2 : 1;
   const int groups = (p.n + 16 * s.rg - 1) / (16 * s.rg);
   // Waves of a group: as many as fill the card, then as few as leave each the same
   // whole rounds of kStreamDepth blocks.
-  const int want = std::min({stream_waves(s.mb, s.rg), p.kblocks(), (2048 + groups * chunks - 1) / (groups * chunks)});
+  const int want = std::min({stream_waves(s.mb), p.kblocks(), (2048 + groups * chunks - 1) / (groups * chunks)});
   int each = (p.kblocks() + want - 1) / want;
   each = (each + kStreamDepth - 1) / kStreamDepth * kStreamDepth;
   const int ks = (p.kblocks() + each - 1) / each;
@@ -410,12 +412,15 @@ static void run_stream(const Fp8Product& p, const ProductOut& out, int kind, con
   else
     fp8_stream_kernel<MB, RG, kOutScores><<<grid, block, t.lds, s>>>(p, out, t.shape);
 }
-template <int RG>
 static void run_stream_rows(const Fp8Product& p, const ProductOut& out, int kind, const StreamPlan& t, hipStream_t s) {
-  if (t.mb == 1) run_stream<1, RG>(p, out, kind, t, s);
-  if (t.mb == 2) run_stream<2, RG>(p, out, kind, t, s);
-  if (t.mb == 3) run_stream<3, RG>(p, out, kind, t, s);
-  if (t.mb == 4) run_stream<4, RG>(p, out, kind, t, s);
+  if (t.rg == 2) {
+    run_stream<4, 2>(p, out, kind, t, s);
+    return;
+  }
+  if (t.mb == 1) run_stream<1, 1>(p, out, kind, t, s);
+  if (t.mb == 2) run_stream<2, 1>(p, out, kind, t, s);
+  if (t.mb == 3) run_stream<3, 1>(p, out, kind, t, s);
+  if (t.mb == 4) run_stream<4, 1>(p, out, kind, t, s);
 }
 
 // ---- few rows and many columns (a vocabulary): persistent workgroups of eight
@@ -659,8 +664,7 @@ static void launch_product(const Fp8Product& p, const ProductOut& out, int kind,
     if (mb == 3) run_wide<3>(p, out, kind, s);
     if (mb == 4) run_wide<4>(p, out, kind, s);
   } else if (takes_stream(p, kind, work_bytes)) {
-    const StreamPlan t = plan_stream(p, kind == kOutScores);
-    t.rg == 2 ? run_stream_rows<2>(p, out, kind, t, s) : run_stream_rows<1>(p, out, kind, t, s);
+    run_stream_rows(p, out, kind, plan_stream(p, kind == kOutScores), s);
   } else {
     launch_fp8_gemm(p, out, kind, work, work_bytes, s);
   }
