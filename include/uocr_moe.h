@@ -412,7 +412,7 @@ int uocr_token_logprobs_async(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype 
  * in registers (scratch: 16 bytes per row and 128 ids, for at most 64 rows per 16
  * ids); alternatives take them through the context's scratch in f32, as many rows
  * at a time as fit (none: Resource). A row with a logit that is not finite gets
- * NaN and raises Numerical; logits in registers may do so from 1e38 on. */
+ * NaN and raises Numerical; logits in registers may do so from 1e9 on. */
 int uocr_fp8_linear_logprobs(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m,
                              size_t k, const uint8_t* w, const float* ws, size_t n,
                              const uocr_token_scores* scores);

@@ -299,6 +299,23 @@ def test_linear_many_rows_of_small_products(ctx, m, n, k):
     test_linear_random(ctx, m, n, k)
 
 
+@pytest.mark.parametrize("m,n,k", [(3, 44, 272), (70, 600, 144), (300, 1280, 2192), (520, 8192, 128), (2, 66000, 144),
+                                   (5, 64, 100)])
+def test_linear_results_at_any_element(ctx, m, n, k):
+    """Results that start one element behind an aligned address, and nothing beside them."""
+    say(f"unaligned result {m}x{n}x{k}")
+    ops = exact_product(m, n, k, m + n)
+    a, b = spread(*ops)
+    want = torch.from_numpy(a @ b.T)
+    dev = device_product(*ops)
+    for dtype in (torch.float32, torch.bfloat16):
+        guard = torch.full((m * n + 2,), 77.0, device="cuda", dtype=dtype)
+        torch.cuda.synchronize()
+        um.fp8_linear(ctx, *dev, guard[1:-1].view(m, n))
+        assert torch.equal(guard[1:-1].view(m, n).cpu(), want.float().to(dtype))
+        assert float(guard[0]) == float(guard[-1]) == 77.0
+
+
 def test_linear_most_rows(ctx):
     """As many rows as a call takes, of one column: whole numbers again."""
     m, k = 1 << 22, 16

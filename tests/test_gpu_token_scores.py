@@ -337,6 +337,28 @@ def test_linear_logprobs_wide(ctx, m, n, k):
     compare(out.host(), want)
 
 
+@pytest.mark.parametrize("m,n", [(2, 500), (200, 3000), (600, 8000), (7, 66000)])
+@pytest.mark.parametrize("offset", [2.0 ** 20, -2.0 ** 22])
+def test_linear_logprobs_of_logits_far_from_zero(ctx, m, n, offset):
+    """Logits offset + whole numbers of some units: the first block is a constant of
+    all words, the second what tells them apart; all sums exact in f32."""
+    say(f"fused scores {m}x{n} around {offset}")
+    rng = np.random.default_rng(m + n)
+    x, w = np.zeros((m, 256)), np.zeros((n, 256))
+    x[:, 0], w[:, 0] = 1, np.sign(offset)
+    x[:, 128:], w[:, 128:] = rng.integers(-1, 2, (m, 128)), rng.integers(-1, 2, (n, 128))
+    scales = np.ones((m, 2), np.float32)
+    scales[:, 0] = abs(offset)
+    ops = [torch.from_numpy(a).to(torch.float8_e4m3fn).cuda() for a in (x, w)]
+    ws = torch.ones((blocks(n), 2), device="cuda")
+    tokens = rng.integers(0, n, m).astype(np.int32)
+    out = Scores(m, 0)
+    torch.cuda.synchronize()
+    um.fp8_linear_logprobs(ctx, ops[0], torch.from_numpy(scales).cuda(), ops[1], ws,
+                           torch.from_numpy(tokens).cuda(), **out.views())
+    compare(out.host(), reference(offset + x[:, 128:] @ w[:, 128:].T, tokens, 0))
+
+
 @pytest.mark.parametrize("m", [3, 200])
 def test_linear_logprobs_errors(ctx, m):
     n, k = 300, 256

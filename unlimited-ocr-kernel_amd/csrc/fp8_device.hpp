@@ -76,9 +76,9 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
     for (int r = 0; r < 4; r++) most = FULL || col + 16 * i + r < n ? fmaxf(most, v[i][r]) : most;
   most = fmaxf(most, __shfl_xor(most, 16));
   most = fmaxf(most, __shfl_xor(most, 32));
-  // d = log2(e) x - r2 in one instruction; r2's rounding, the same for all of the row's
-  // logits here, is put right at the end (2^c = 1 + c ln 2 for a c of some 1e-6).
-  // Logits past 1e38, whose r2 would overflow, end as an infinite sum.
+  // d = log2(e) x - r2 in one instruction; r2's rounding c, the same for all of the
+  // row's logits here, is put right at the end: the terms are 2^(d + c). Beyond 1e9 c is
+  // large enough for 2^c to overflow or vanish, which ends as a row without distribution.
   q.r = fminf(fmaxf(most, -1e38f), 1e38f);
   const float r2 = q.r * kLog2e;
 #pragma unroll
@@ -105,9 +105,9 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
     q.t += __shfl_xor(q.t, o);
   }
   const float c = fmaf(-q.r, kLog2e, r2);
-  q.t = fmaf(q.s, c, q.t);
-  q.t = fmaf(q.t, c * kLn2, q.t);
-  q.s = fmaf(q.s, c * kLn2, q.s);
+  const float e = __builtin_amdgcn_exp2f(c);
+  q.t = fmaf(q.s, c, q.t) * e;
+  q.s *= e;
   return q;
 }
 // The same, whether or not the wave's columns (from n0 on) end below n.
