@@ -554,19 +554,23 @@ def _whole(t, shape, code: int, device: int) -> bool:
 
 def _rows(t, device: int, what: str):
     """(rows, columns, row stride) of a 2-D tensor whose rows are contiguous."""
-    if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1) or t.get_device() != device:
+    shape = t.shape
+    if len(shape) != 2 or t.get_device() != device:
         _refuse(f"{what} must be rows on the context's device")
-    rows, cols = t.shape
-    return rows, cols, t.stride(0) if rows > 1 else max(cols, 1)
+    rows, cols = shape
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
+        _refuse(f"{what} must be rows of adjacent elements")
+    return rows, cols, ld if rows > 1 else max(cols, 1)
 
 
 def _quantize(fn, ctx, x, q, scales, tile: int):
-    device = ctx.device
-    rows, cols, ld = _rows(x, device, "x")
-    if not _whole(q, (rows, cols), _FP8, device):
-        _refuse("q must be contiguous e4m3 bytes of x's shape, on the context's device")
-    if not _whole(scales, (-(-rows // tile), -(-cols // 128)), 2, device):
-        _refuse("scales must be f32, one per block, on the context's device")
+    rows, cols, ld = _rows(x, ctx.device, "x")
+    if q.shape != (rows, cols) or scales.shape != ((rows + tile - 1) // tile, (cols + 127) // 128):
+        _refuse("q must have x's shape, scales one element per block")
+    if not (_types[q.dtype] == _FP8 and _types[scales.dtype] == 2 and q.is_contiguous() and scales.is_contiguous()
+            and q.get_device() == scales.get_device() == ctx.device):
+        _refuse("q and scales must be contiguous e4m3 bytes and f32 on the context's device")
     status = fn(ctx.handle, x.data_ptr(), _type(x), rows, cols, ld, q.data_ptr(),
                 scales.data_ptr())
     if status:
@@ -576,7 +580,7 @@ def _quantize(fn, ctx, x, q, scales, tile: int):
 def fp8_quantize(ctx: Context, x, q, scales, sync: bool = True):
     """Rows x [rows, cols] (f32 or bf16, any row stride) to e4m3 q [rows, cols]
     (float8_e4m3fn or uint8) and f32 scales [rows, ceil(cols / 128)]."""
-    _quantize(_operator("uocr_fp8_quantize", sync), ctx, x, q, scales, 1)
+    _quantize(_bound.get(("uocr_fp8_quantize", sync)) or _operator("uocr_fp8_quantize", sync), ctx, x, q, scales, 1)
 
 
 def fp8_quantize_weight(ctx: Context, w, q, scales):
@@ -609,7 +613,8 @@ def fp8_linear(ctx: Context, xq, xs, wq, ws, y, sync: bool = True):
     args = _product(ctx, xq, xs, wq, ws)
     if y.shape != (args[2], args[6]) or not y.is_contiguous() or y.get_device() != ctx.device:
         _refuse("y must be [m, n] on the context's device")
-    status = _operator("uocr_fp8_linear", sync)(ctx.handle, *args, y.data_ptr(), _type(y))
+    fn = _bound.get(("uocr_fp8_linear", sync)) or _operator("uocr_fp8_linear", sync)
+    status = fn(ctx.handle, *args, y.data_ptr(), _type(y))
     if status:
         _check(status)
 
