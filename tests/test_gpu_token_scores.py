@@ -99,7 +99,7 @@ def logits_of(rng, rows, vocab, dtype):
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 # Vocabularies around a vector, a group of columns, a chunk, and the decoder's.
 SIZES = [(1, 1), (3, 2), (2, 7), (5, 63), (4, 64), (3, 65), (7, 129), (2, 1023), (2, 1025), (300, 1000),
-         (9, 4099), (2, 16385), (1, 129280), (40, 40001)]
+         (9, 4099), (2, 16385), (1, 129280), (40, 40001), (3, 8192), (3, 8193), (600, 200), (65, 9000)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
@@ -120,12 +120,14 @@ def test_token_logprobs(ctx, rows, vocab, dtype):
             compare(out.host(), want)
 
 
+# Vocabularies of one launch per row, and of two.
+@pytest.mark.parametrize("vocab", [3001, 20001])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-def test_banned_ids_and_ties(ctx, dtype):
+def test_banned_ids_and_ties(ctx, dtype, vocab):
     """-inf is probability 0 (a banned given token: -inf); equal logits by rising
     id, -0 equal to 0; the lowest finite value is a logit like others."""
     rng = np.random.default_rng(5)
-    rows, vocab = 12, 3001
+    rows = 12
     x = logits_of(rng, rows, vocab, dtype)
     x[:, rng.random(vocab) < 0.5] = -math.inf
     x[1] = 0.0
@@ -170,12 +172,13 @@ def test_far_spread_logits(ctx):
     compare(out.host(), want)
 
 
+@pytest.mark.parametrize("vocab", [700, 12300])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
-def test_rows_without_a_distribution(ctx, dtype):
+def test_rows_without_a_distribution(ctx, dtype, vocab):
     """NaN, +inf and rows with no finite logit raise Numerical and get NaN and ids
     -1; the rows beside them are right; padding rows may hold anything."""
     rng = np.random.default_rng(7)
-    rows, vocab, top = 9, 700, 4
+    rows, top = 9, 4
     x = logits_of(rng, rows, vocab, dtype)
     good = x.clone()
     x[1, 699] = math.nan
@@ -594,7 +597,8 @@ def test_head_refusals(ctx):
     head.close()
 
 
-def test_scores_in_a_graph(ctx):
+@pytest.mark.parametrize("vocab", [4000, 20000])
+def test_scores_in_a_graph(ctx, vocab):
     """Captured scoring replays with the eager bits, eager work in between; the
     logits change between replays."""
     rng = np.random.default_rng(11)
@@ -604,7 +608,7 @@ def test_scores_in_a_graph(ctx):
     torch.cuda.synchronize()
     um.fp8_quantize_weight(ctx, weight, wq, ws)
     head = um.LmHead(ctx, norm, 1e-6, q=wq, scales=ws, mode=um.QUANT_FP8_BLOCKS, where=um.MEMORY_DEVICE)
-    x = logits_of(rng, 33, 4000, torch.bfloat16).cuda()
+    x = logits_of(rng, 33, vocab, torch.bfloat16).cuda()
     got, want = [Scores(33, 0), Scores(33, 5), Scores(33, 5)], [Scores(33, 0), Scores(33, 5), Scores(33, 5)]
 
     def work(out, sync):

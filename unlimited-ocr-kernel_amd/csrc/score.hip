@@ -104,6 +104,26 @@ __device__ __forceinline__ float row16_max(float v) {
   return v;
 }
 
+// A lane's statistics of its values, with the reference `most`, which none is above.
+template <int V, int VEC>
+__device__ __forceinline__ ScorePart lane_statistics(const float (&v)[V][VEC], float most) {
+  // Banned words only have no reference; with 0 in its place every term vanishes (and
+  // a NaN stays one).
+  const float r = most == -INFINITY ? 0.0f : most;
+  float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < V; i++)
+#pragma unroll
+    for (int j = 0; j < VEC; j++) {
+      // A banned word's distance is brought to where 2^d is 0 and 0 times d too.
+      const float d = (v[i][j] - r) * kLog2e;
+      const float e = __builtin_amdgcn_exp2f(d);
+      s[j & 1] += e;
+      t[j & 1] = fmaf(e, fmaxf(d, -1000.0f), t[j & 1]);
+    }
+  return {most, s[0] + s[1], t[0] + t[1], 0.0f};
+}
+
 template <typename T, int V>
 __global__ __launch_bounds__(kScoreThreads) void score_chunks_kernel(
     const T* __restrict__ logits, size_t items, int vocab, size_t ld, const int32_t* __restrict__ tokens,
@@ -134,25 +154,10 @@ __global__ __launch_bounds__(kScoreThreads) void score_chunks_kernel(
   }
   most = fmaxf(most, __shfl_xor(most, 16));
   most = fmaxf(most, __shfl_xor(most, 32));
-  ScorePart p = empty_part();
-  p.r = most;
-  // A chunk of banned words has no reference; with 0 in its place every term
-  // vanishes (and a NaN stays one).
-  const float r = most == -INFINITY ? 0.0f : most;
-  float s[2] = {0.0f, 0.0f}, t[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int i = 0; i < V; i++)
-#pragma unroll
-    for (int j = 0; j < kVec; j++) {
-      // A banned word's distance is brought to where 2^d is 0 and 0 times d too.
-      const float d = (v[i][j] - r) * kLog2e;
-      const float e = __builtin_amdgcn_exp2f(d);
-      s[j & 1] += e;
-      t[j & 1] = fmaf(e, fmaxf(d, -1000.0f), t[j & 1]);
-    }
+  ScorePart p = lane_statistics<V, kVec>(v, most);
   auto add = [](float a, float b) { return a + b; };
-  p.s = lanes_reduce<1>(s[0] + s[1], add);
-  p.t = lanes_reduce<1>(t[0] + t[1], add);
+  p.s = lanes_reduce<1>(p.s, add);
+  p.t = lanes_reduce<1>(p.t, add);
   if (lane == 0) parts[item] = p;
 }
 
@@ -175,16 +180,29 @@ constexpr int kMostGroups = 512, kMostCandidates = 1024;
 // Group maxima that a thread keeps in registers (rows of up to 131072 or 262144
 // logits); those of longer rows are read twice.
 constexpr int kHeldMaxima = 8;
+constexpr int kScorer = kScoreThreads - 64;  // first thread of the last wave, which writes a row's scores
 
+// What a padding row gets.
+__device__ __forceinline__ void write_padding(const TokenScores& out, size_t row, int tid) {
+  if (tid == 0 && out.logprobs) out.logprobs[row] = 0.0f;
+  if (tid == 0 && out.entropy) out.entropy[row] = 0.0f;
+  for (int i = tid; i < out.top; i += kScoreThreads) {
+    out.top_ids[row * out.top + i] = -1;
+    out.top_logprobs[row * out.top + i] = -INFINITY;
+  }
+}
+
+// A row's outputs from its threads' statistics p and its groups' maxima, of which g are
+// this thread's first and group_max(at) gives any. `most` is the largest of some logits
+// of this thread's own, which the first `filled` threads have; `given` the given token's
+// logit in the last wave's first thread.
 // A chain of dependent reads (the maxima; then the candidates' logits) and barriers,
 // which is what it takes: everything that can be read early is, and nothing that can
-// wait stands before a barrier. One row of 129280 f32 6.1 us: 1.7 to the maxima, 0.7 to
-// tau, 0.6 to the list, 1.2 to the candidates, 0.5 to the ranks.
-template <typename T>
-__global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
-    const T* __restrict__ logits, int vocab, size_t ld, int chunks,
-    const ScorePart* __restrict__ parts, const float* __restrict__ maxima, int groups,
-    TokenScores out, int* err) {
+// wait stands before a barrier.
+template <typename T, class GroupMax>
+__device__ __forceinline__ void finish_row(const T* x, size_t row, int vocab, int groups, ScorePart p,
+                                           const float (&g)[kHeldMaxima], const GroupMax& group_max, float most,
+                                           int filled, int token, float given, const TokenScores& out, int* err) {
   constexpr int kVec = Logits<T>::kVec, kGroup = 16 * kVec;
   __shared__ ScorePart held[kScoreThreads / 64];
   __shared__ unsigned long long keys[kMostCandidates];
@@ -194,40 +212,10 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   __shared__ int counts[2];
   __shared__ float normalizer[2];
   __shared__ bool good;
-  const size_t row = blockIdx.x;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int top = out.top;
-  const float* gmax = maxima + row * groups;
-  float g[kHeldMaxima];
-#pragma unroll
-  for (int i = 0; i < kHeldMaxima; i++) {
-    const int at = tid + i * kScoreThreads;
-    g[i] = top && at < groups ? gmax[at] : -INFINITY;
-  }
-  ScorePart p = empty_part();
-  for (int c = tid; c < chunks; c += kScoreThreads) p = join(p, parts[row * chunks + c]);
-  const int token = out.tokens ? out.tokens[row] : 0;
-  if (token < 0) {  // a padding row; what was read of it is not used
-    if (tid == 0 && out.logprobs) out.logprobs[row] = 0.0f;
-    if (tid == 0 && out.entropy) out.entropy[row] = 0.0f;
-    for (int i = tid; i < top; i += kScoreThreads) {
-      out.top_ids[row * top + i] = -1;
-      out.top_logprobs[row * top + i] = -INFINITY;
-    }
-    return;
-  }
-  const T* x = logits + row * ld;
-  constexpr int kScorer = kScoreThreads - 64;  // first thread of the last wave
-  const float given = tid == kScorer && out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f;
-  // This thread's largest group.
-  float most = g[0];
-#pragma unroll
-  for (int i = 1; i < kHeldMaxima; i++) most = fmaxf(most, g[i]);
-  if (top)
-    for (int at = tid + kHeldMaxima * kScoreThreads; at < groups; at += kScoreThreads) most = fmaxf(most, gmax[at]);
   // tau is chosen from the maxima of four, two or single threads each: fewer to rank,
   // as long as they are as many as the alternatives.
-  const int filled = min(groups, kScoreThreads);
   const int share = 4 * top <= filled ? 4 : 2 * top <= filled ? 2 : 1;
   if (share >= 2) most = fmaxf(most, dpp_move<0xB1>(most));
   if (share == 4) most = fmaxf(most, dpp_move<0x4E>(most));
@@ -249,8 +237,8 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
     }
     if (larger < top) atomicMin(&tau_at, (uint32_t)(order_key(v, 0) >> 32));
   }
-  // The last wave, which has no maximum to rank where four threads share one, joins
-  // the waves' statistics meanwhile.
+  // The last wave, which has no maximum to rank where threads share one, joins the
+  // waves' statistics meanwhile.
   if (tid >= kScorer) {
     p = lanes_join<1>(lane < kScoreThreads / 64 ? held[lane] : empty_part());
     if (lane == 0) {
@@ -280,7 +268,7 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   };
 #pragma unroll
   for (int i = 0; i < kHeldMaxima; i++) list(tid + i * kScoreThreads, g[i]);
-  for (int at = tid + kHeldMaxima * kScoreThreads; at < groups; at += kScoreThreads) list(at, gmax[at]);
+  for (int at = tid + kHeldMaxima * kScoreThreads; at < groups; at += kScoreThreads) list(at, group_max(at));
   __syncthreads();
   const int some = counts[0];
   if (some <= kMostGroups) {
@@ -340,11 +328,104 @@ __global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
   }
 }
 
+// One row of 129280 f32 6.1 us: 1.7 to the maxima, 0.7 to tau, 0.6 to the list, 1.2 to
+// the candidates, 0.5 to the ranks.
+template <typename T>
+__global__ __launch_bounds__(kScoreThreads) void score_rows_kernel(
+    const T* __restrict__ logits, int vocab, size_t ld, int chunks,
+    const ScorePart* __restrict__ parts, const float* __restrict__ maxima, int groups,
+    TokenScores out, int* err) {
+  const size_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const float* gmax = maxima + row * groups;
+  float g[kHeldMaxima];
+#pragma unroll
+  for (int i = 0; i < kHeldMaxima; i++) {
+    const int at = tid + i * kScoreThreads;
+    g[i] = out.top && at < groups ? gmax[at] : -INFINITY;
+  }
+  ScorePart p = empty_part();
+  for (int c = tid; c < chunks; c += kScoreThreads) p = join(p, parts[row * chunks + c]);
+  const int token = out.tokens ? out.tokens[row] : 0;
+  if (token < 0) {  // what was read of it is not used
+    write_padding(out, row, tid);
+    return;
+  }
+  const T* x = logits + row * ld;
+  const float given = tid == kScorer && out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f;
+  float most = g[0];
+#pragma unroll
+  for (int i = 1; i < kHeldMaxima; i++) most = fmaxf(most, g[i]);
+  if (out.top)
+    for (int at = tid + kHeldMaxima * kScoreThreads; at < groups; at += kScoreThreads) most = fmaxf(most, gmax[at]);
+  finish_row<T>(x, row, vocab, groups, p, g, [&](int at) { return gmax[at]; }, most, min(groups, kScoreThreads), token,
+                given, out, err);
+}
+
+// Short rows (up to kWholeVocab logits) are read by the workgroup that finishes them: no
+// second launch, the groups' maxima stay in LDS, and tau comes from every thread's logits,
+// which are more than the groups. 61 x 5000 f32 8.2 -> 7.2 us, 512 x 8192 bf16 10.4 ->
+// 8.1; with 20 alternatives 61 x 1000 f32 65 -> 7.1 (fewer groups than alternatives). 61
+// x 12000 would be 6% faster too, 61 x 16384 not, 61 x 129280 39 us against 14.7.
+constexpr int kWholeVectors = 4, kWholeVocab = 8192;
+template <typename T>
+__global__ __launch_bounds__(kScoreThreads) void score_short_rows_kernel(const T* __restrict__ logits, int vocab,
+                                                                         size_t ld, int groups, TokenScores out,
+                                                                         int* err) {
+  constexpr int kVec = Logits<T>::kVec, V = kWholeVectors;
+  __shared__ float gmax[kWholeVocab / (16 * kVec)];
+  const size_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int token = out.tokens ? out.tokens[row] : 0;
+  if (token < 0) {  // not read
+    write_padding(out, row, tid);
+    return;
+  }
+  const T* x = logits + row * ld;
+  const float given = tid == kScorer && out.logprobs && token < vocab ? Logits<T>::widen(x[token]) : 0.0f;
+  ScorePart p = empty_part();
+  float largest = -INFINITY;
+  // Whole waves: row16_max reads all sixteen lanes.
+  for (int c0 = tid * kVec; c0 - lane * kVec < vocab; c0 += kScoreThreads * V * kVec) {
+    float v[V][kVec];
+#pragma unroll
+    for (int i = 0; i < V; i++) load_logits<T>(x, c0 + i * kScoreThreads * kVec, vocab, v[i]);
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      float m = v[i][0];
+#pragma unroll
+      for (int j = 1; j < kVec; j++) m = fmaxf(m, v[i][j]);
+      most = fmaxf(most, m);
+      if (out.top) {
+        m = row16_max(m);
+        const int c = c0 + i * kScoreThreads * kVec;
+        if ((lane & 15) == 0 && c < vocab) gmax[c / (16 * kVec)] = m;
+      }
+    }
+    p = join(p, lane_statistics<V, kVec>(v, most));
+    largest = fmaxf(largest, most);
+  }
+  __syncthreads();
+  float g[kHeldMaxima];
+#pragma unroll
+  for (int i = 0; i < kHeldMaxima; i++) {
+    const int at = tid + i * kScoreThreads;
+    g[i] = out.top && at < groups ? gmax[at] : -INFINITY;
+  }
+  finish_row<T>(x, row, vocab, groups, p, g, [&](int at) { return gmax[at]; }, largest,
+                min((vocab + kVec - 1) / kVec, kScoreThreads), token, given, out, err);
+}
+
 template <typename T>
 static void launch(const T* logits, size_t rows, int vocab, size_t ld, const ScorePlan& plan,
                    const TokenScores& out, void* work, int* err, hipStream_t s) {
   auto* parts = static_cast<ScorePart*>(work);
   float* maxima = out.top ? reinterpret_cast<float*>(static_cast<char*>(work) + plan.maxima_at) : nullptr;
+  if (vocab <= kWholeVocab) {
+    score_short_rows_kernel<T><<<(unsigned)rows, kScoreThreads, 0, s>>>(logits, vocab, ld, plan.groups, out, err);
+    return;
+  }
   const size_t items = rows * plan.chunks;
   const dim3 grid((unsigned)((items + kScoreThreads / 64 - 1) / (kScoreThreads / 64))), block(kScoreThreads);
 #define UOCR_CHUNKS(V)                                                                             \
