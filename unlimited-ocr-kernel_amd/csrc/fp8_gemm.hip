@@ -118,19 +118,24 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 // per scale block, at twice the rate. Either way a block's sum is scaled into the f32
 // accumulators when it is done.
 //
-// BUFS stages of LDS, so that two workgroups share a CU and hide each other's waits: two
-// stages with tiles of 128 rows, three with tiles of 64. Where there are no more tiles of
-// 128 than CUs, those of 64 are taken: more of them, less padding, and a stage more in
-// flight (277 x 1280 x 6848 f32 20.9 -> 17.3 us, 1024 x 1280 x 896 bf16 9.6 -> 7.1; beyond,
-// 1024 x 6848 x 1280 bf16 is 18.4 us with 128 rows and 21.8 with 64). Few tiles of a long
-// depth are also split along it: each split leaves f32 partial sums in memory, and a
-// second launch adds them in order.
+// BUFS stages of LDS, so that workgroups share a CU and hide each other's waits: two
+// stages with tiles of 128 rows, two workgroups to a CU; with tiles of 64 rows two stages
+// and three workgroups (WIDEN: 600 x 6848 x 1280 scores 24.2 us with three stages, 21.2
+// with two), or three stages and two workgroups (bf16 results, whose steps are shorter:
+// 2048 x 1280 x 6848 41 and 43.5 us). The smaller tiles are taken where all of them fit
+// the card at once: more of them, less padding (277 x 1280 x 6848 f32 20.9 -> 16.8 us,
+// 1024 x 1280 x 896 bf16 9.6 -> 7.1, 3500 x 1280 x 6848 f32 100 -> 92; beyond, 1024 x
+// 6848 x 1280 f32 is 26.7 us with 128 rows and 29.9 with 64). Few tiles of a long depth
+// are also split along it: each split leaves f32 partial sums in memory, and a second
+// launch adds them in order.
 //
 // 4096 x 6848 x 1280 bf16 55 us (1310 TFLOP/s): the loads bring 17 TB/s into LDS, which is
 // what bounds the steps, and the stores take 10 us. 4096 x 129280 x 1280 scores 1275 us
 // (1060 TFLOP/s): the vector instructions, 3.4 a product (2 of widening, 1 of scaling) and
 // the statistics', share the issue with the products.
 constexpr int kCols = 128;  // columns of a tile
+constexpr int short_bufs(bool widen) { return widen ? 2 : 3; }
+constexpr int short_per_cu(bool widen) { return widen ? 3 : 2; }
 constexpr int tile_rows(int xb) { return 32 * xb; }  // for xb blocks of 16 rows in each of two waves
 constexpr uint32_t stage_bytes(int xb) { return (tile_rows(xb) + kCols) * 128u; }
 // Scales of eight blocks: x's [8][rows of the tile], the matrix's [8].
@@ -417,18 +422,25 @@ static void run_tall(const Fp8Product& p, const ProductOut& out, hipStream_t s) 
 }
 template <bool WIDEN, int OUT>
 static void run_short(const Fp8Product& p, const ProductOut& out, const Splits& splits, hipStream_t s) {
-  run_tiles<WIDEN, OUT, 3, 2>(p, out, splits, s);
+  run_tiles<WIDEN, OUT, short_bufs(WIDEN), 2>(p, out, splits, s);
 }
 
-static bool takes_tall(const Fp8Product& p) { return tiles_of(p, tile_rows(4)) > (size_t)kCus; }
+// Short tiles are taken as long as they all fit the card at once.
+static bool takes_tall(const Fp8Product& p, bool widen) {
+  return tiles_of(p, tile_rows(2)) > (size_t)short_per_cu(widen) * kCus;
+}
 
 // A model of the time in units of 0.1 us, with what was measured for its parts: a
 // workgroup's start and end 35; a step of one that has a CU to itself 7.7 (WIDEN) or 4.5,
-// of two that share one 12 or 7; with tall tiles twice that.
+// of two that share one 12 or 7, of three 17; with tall tiles twice that.
 static double tiles_time(size_t workgroups, int steps, bool widen, bool tall) {
-  const double size = tall ? 2.0 : 1.0, alone = size * (widen ? 7.7 : 4.5), shared = size * (widen ? 12.0 : 7.0);
-  const size_t full = workgroups / (2 * kCus), rest = workgroups % (2 * kCus);
-  return full * (35 + shared * steps) + (rest ? 35 + (rest > (size_t)kCus ? shared : alone) * steps : 0.0);
+  static const double kStep[2][3] = {{4.5, 7.0, 0.0}, {7.7, 12.0, 17.0}};
+  const int most = tall ? 2 : short_per_cu(widen);
+  const size_t full = workgroups / (most * kCus), rest = workgroups % (most * kCus);
+  const double unit = steps * (tall ? 2.0 : 1.0);
+  double time = full * (35 + kStep[widen][most - 1] * unit);
+  if (rest) time += 35 + kStep[widen][(rest - 1) / kCus] * unit;
+  return time;
 }
 
 // How many ways to split the depth, and the modelled time: the second launch takes 30 and
@@ -452,8 +464,8 @@ static TilePlan plan_splits(const Fp8Product& p, bool widen, size_t work_bytes) 
 }
 
 double fp8_gemm_time(const Fp8Product& p, bool widen, size_t work_bytes) {
-  return takes_tall(p) ? tiles_time(tiles_of(p, tile_rows(4)), p.kblocks(), widen, true)
-                       : plan_splits(p, widen, work_bytes).time;
+  return takes_tall(p, widen) ? tiles_time(tiles_of(p, tile_rows(4)), p.kblocks(), widen, true)
+                              : plan_splits(p, widen, work_bytes).time;
 }
 
 int fp8_gemm_parts(const Fp8Product& p) {
@@ -469,10 +481,10 @@ void fp8_gemm_init_attributes() {
   tile_attributes<false, kOutBf16, 2, 4>();
   tile_attributes<true, kOutF32, 2, 4>();
   tile_attributes<true, kOutScores, 2, 4>();
-  tile_attributes<false, kOutBf16, 3, 2>();
-  tile_attributes<false, kOutF32, 3, 2>();
-  tile_attributes<true, kOutF32, 3, 2>();
-  tile_attributes<true, kOutScores, 3, 2>();
+  tile_attributes<false, kOutBf16, short_bufs(false), 2>();
+  tile_attributes<false, kOutF32, short_bufs(false), 2>();
+  tile_attributes<true, kOutF32, short_bufs(true), 2>();
+  tile_attributes<true, kOutScores, short_bufs(true), 2>();
 }
 
 void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
@@ -487,7 +499,7 @@ void launch_fp8_gemm(const Fp8Product& p, const ProductOut& out, int kind, void*
       fp8_bytes_kernel<kOutScores><<<grid, 256, 0, s>>>(p, out);
     return;
   }
-  if (takes_tall(p)) {
+  if (takes_tall(p, kind != kOutBf16)) {
     if (kind == kOutF32)
       run_tall<true, kOutF32>(p, out, s);
     else if (kind == kOutBf16)
