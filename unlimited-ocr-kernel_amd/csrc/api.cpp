@@ -1342,21 +1342,38 @@ int scratch_fail(uocr_gpu_ctx* ctx) {
 }
 
 // Bytes of score work for `rows` rows of logits or of a product; n_top > 0
-// brings the product's logits into scratch too.
+// brings the product's logits into scratch too. Products of rows that are not whole
+// 16-byte chunks are packed first where there is room.
 size_t logits_need(size_t rows, size_t vocab, const uocr_token_scores& s) {
   return align256(rows * vocab * 4) +
          align256(uocr::token_score_bytes(rows, (int)vocab, uocr::kTypeF32, (int)s.n_top));
 }
-size_t product_need(const uocr::Fp8Product& p, size_t rows, const uocr_token_scores& s) {
+size_t product_need(const uocr::Fp8Product& p, size_t rows, const uocr_token_scores& s, bool pack) {
   uocr::Fp8Product q = p;
   q.m = (int)rows;
-  return s.n_top ? logits_need(rows, p.n, s) : align256(uocr::fp8_score_bytes(q));
+  const size_t copy = pack ? uocr::fp8_pack_bytes(q) : 0;
+  if (copy) q.x = q.w = nullptr, q.k = (q.k + 15) / 16 * 16;  // as the copy has them
+  return copy + (s.n_top ? logits_need(rows, p.n, s) : align256(uocr::fp8_score_bytes(q)));
+}
+// Rows that fit: of a packed product, or where that leaves few or none, of one that is
+// not. need(rows, pack).
+template <class Need>
+size_t product_rows_that_fit(size_t m, size_t limit, const Need& need, bool* pack) {
+  *pack = true;
+  const size_t rows = rows_that_fit(m, limit, [&](size_t r) { return need(r, true); });
+  if (rows >= std::min<size_t>(m, 64)) return rows;
+  *pack = false;
+  return rows_that_fit(m, limit, [&](size_t r) { return need(r, false); });
 }
 
 // Scores rows [row, row + p.m) of the caller's arrays from the product p, in
 // the scratch at `work` (product_need bytes).
-void enqueue_product_scores(uocr_gpu_ctx* ctx, const uocr::Fp8Product& p, char* work,
-                            const uocr_token_scores& s, size_t row) {
+void enqueue_product_scores(uocr_gpu_ctx* ctx, uocr::Fp8Product p, char* work, const uocr_token_scores& s,
+                            size_t row, bool pack) {
+  if (const size_t copy = pack ? uocr::fp8_pack_bytes(p) : 0) {
+    p = uocr::launch_fp8_pack(p, work, ctx->stream);
+    work += copy;
+  }
   const uocr::TokenScores o = scores_from(s, row);
   if (s.n_top) {
     uocr::launch_fp8_linear(p, work, uocr::kTypeF32, nullptr, 0, ctx->stream);
@@ -1414,8 +1431,15 @@ int uocr_fp8_linear_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, 
   if (m == 0) return UOCR_OK;
   if (!y) return fail(UOCR_ERR_SHAPE, "null pointer");
   HIP_TRY(hipSetDevice(ctx->device), "set device");
-  uocr::launch_fp8_linear({x, xs, w, ws, (int)m, (int)n, (int)k}, y, ytype, ctx->scratch, ctx->scratch_limit,
-                          ctx->stream);
+  uocr::Fp8Product p{x, xs, w, ws, (int)m, (int)n, (int)k};
+  char* work = ctx->scratch;
+  size_t bytes = ctx->scratch_limit;
+  if (const size_t copy = uocr::fp8_pack_bytes(p); copy && copy <= bytes) {
+    p = uocr::launch_fp8_pack(p, work, ctx->stream);
+    work += copy;
+    bytes -= copy;
+  }
+  uocr::launch_fp8_linear(p, y, ytype, work, bytes, ctx->stream);
   HIP_TRY(hipGetLastError(), "kernel launch");
   return UOCR_OK;
 }
@@ -1465,15 +1489,16 @@ int uocr_fp8_linear_logprobs_async(uocr_gpu_ctx* ctx, const uint8_t* x, const fl
   if (m == 0) return UOCR_OK;
   HIP_TRY(hipSetDevice(ctx->device), "set device");
   uocr::Fp8Product p{x, xs, w, ws, (int)m, (int)n, (int)k};
+  bool pack;
   const size_t step = std::min(
-      rows_that_fit(m, ctx->scratch_limit, [&](size_t r) { return product_need(p, r, *scores); }),
+      product_rows_that_fit(m, ctx->scratch_limit, [&](size_t r, bool c) { return product_need(p, r, *scores, c); }, &pack),
       uocr::token_score_rows((int)n, uocr::kTypeF32));
   if (!step) return scratch_fail(ctx);
   for (size_t r = 0; r < m; r += step) {
     p.x = x + r * k;
     p.xs = xs + r * p.kblocks();
     p.m = (int)std::min(step, m - r);
-    enqueue_product_scores(ctx, p, ctx->scratch, *scores, r);
+    enqueue_product_scores(ctx, p, ctx->scratch, *scores, r, pack);
     HIP_TRY(hipGetLastError(), "kernel launch");
   }
   return UOCR_OK;
@@ -1674,12 +1699,13 @@ int uocr_lm_head_logprobs_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, con
   // One row under DynamicActivations is projected W8A8, from a quantised copy.
   const bool w8a8 = v.kind == 2 && T == 1;
   const size_t row8 = w8a8 ? align256(H) + align256((H + 31) / 32 * 4) : 0;
-  auto need = [&](size_t rows) {
+  auto need = [&](size_t rows, bool pack) {
     const size_t head_bytes = head_rows(nullptr, v, rows).bytes;
-    return head_bytes + row8 + (fp8 ? product_need(fp8_head(v, {}, rows), rows, *scores)
+    return head_bytes + row8 + (fp8 ? product_need(fp8_head(v, {}, rows), rows, *scores, pack)
                                     : logits_need(rows, V, *scores));
   };
-  const size_t step = std::min({rows_that_fit(T, ctx->scratch_limit, need),
+  bool pack;
+  const size_t step = std::min({product_rows_that_fit(T, ctx->scratch_limit, need, &pack),
                                 uocr::token_score_rows(v.V, uocr::kTypeF32),
                                 fp8 ? product_rows(V) : linear_rows(V, H)});
   if (!step) return scratch_fail(ctx);
@@ -1691,7 +1717,7 @@ int uocr_lm_head_logprobs_async(uocr_gpu_ctx* ctx, const uocr_lm_head* head, con
     char* work = ctx->scratch + h.bytes;
     if (fp8) {
       quantized_head_rows(ctx, v, in, rows, h, tokens);
-      enqueue_product_scores(ctx, fp8_head(v, h, rows), work, *scores, t);
+      enqueue_product_scores(ctx, fp8_head(v, h, rows), work, *scores, t, pack);
     } else {
       float* logits = reinterpret_cast<float*>(work);
       char* after = work + align256(rows * V * 4);

@@ -33,6 +33,11 @@ struct Fp8Product {
   int m, n, k;
   __host__ __device__ int kblocks() const { return (k + kFp8Block - 1) / kFp8Block; }
 };
+// Rows of whole 16-byte chunks at aligned addresses, which the fast kernels take. Where p's
+// are not, a copy of both operands that are, with zeros behind each row's end: its bytes
+// (0 where it needs none), and the launch that makes it at `work` (256-byte aligned).
+size_t fp8_pack_bytes(const Fp8Product& p);
+Fp8Product launch_fp8_pack(const Fp8Product& p, void* work, hipStream_t s);
 // `work`: room for partial sums where the depth is split; any size will do.
 void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, void* work, size_t work_bytes, hipStream_t s);
 

@@ -21,9 +21,37 @@ __device__ __forceinline__ uint4 load_chunk(const uint8_t* row, int k, int K) {
   return v;
 }
 
-// The product of rows whose bytes may start at any address (K no multiple of 16):
-// 128 x 128 outputs per workgroup of four waves, 64 x 64 each, staged through
-// registers. Not tuned.
+// Both operands with rows of whole chunks, a chunk per thread. 4096 x 6848 x 1279 f32:
+// 219 us on the kernel below, 102 on tiles of such a copy; 1 x 1280 x 6847 142 and 14.
+__global__ __launch_bounds__(256) void fp8_pack_kernel(Fp8Product p, uint8_t* __restrict__ x, uint8_t* __restrict__ w) {
+  const uint32_t chunks = (p.k + 15) / 16, all_x = p.m * chunks, all = all_x + p.n * chunks;
+  uint32_t c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= all) return;
+  const bool second = c >= all_x;
+  if (second) c -= all_x;
+  const uint4 v = load_chunk((second ? p.w : p.x) + (size_t)(c / chunks) * p.k, (int)(c % chunks) * 16, p.k);
+  reinterpret_cast<uint4*>(second ? w : x)[c] = v;
+}
+
+// A thread per chunk, counted in 32 bits: larger copies have no room anywhere.
+constexpr size_t kMostPacked = (size_t)1 << 35;
+static size_t pack_part(int rows, int k) { return ((size_t)rows * ((k + 15) / 16) * 16 + 255) / 256 * 256; }
+size_t fp8_pack_bytes(const Fp8Product& p) {
+  if (whole_chunks(p)) return 0;
+  const size_t bytes = pack_part(p.m, p.k) + pack_part(p.n, p.k);
+  return bytes < kMostPacked ? bytes : SIZE_MAX / 2;
+}
+Fp8Product launch_fp8_pack(const Fp8Product& p, void* work, hipStream_t s) {
+  auto* x = static_cast<uint8_t*>(work);
+  uint8_t* w = x + pack_part(p.m, p.k);
+  const size_t chunks = ((size_t)p.m + p.n) * ((p.k + 15) / 16);
+  fp8_pack_kernel<<<(unsigned)((chunks + 255) / 256), 256, 0, s>>>(p, x, w);
+  return {x, p.xs, w, p.ws, p.m, p.n, (p.k + 15) / 16 * 16};
+}
+
+// The product of rows whose bytes may start at any address (K no multiple of 16), where
+// there is no room for a copy: 128 x 128 outputs per workgroup of four waves, 64 x 64
+// each, staged through registers. Not tuned.
 template <int OUT>
 __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut out) {
   constexpr int kT = 128;
