@@ -372,8 +372,10 @@ int uocr_fp8_quantize_weight(uocr_gpu_ctx* ctx, const void* w, uocr_dtype type, 
  * eight products (some 1e-5 of a sum, at most 2^-10 of the sum of magnitudes);
  * F32 results keep all bits. A NaN byte makes its row or column NaN and raises
  * nothing. Works in the context's scratch: long depths of few rows and columns are
- * split, as far as the partial sums fit. Equal calls give equal bits; a row's last
- * bits depend on m and on the scratch limit, which choose how its sums are split.
+ * split, as far as the partial sums fit, and rows of many whose k is no multiple of
+ * 16 (or that start at no multiple of 16) are copied first, where both matrices fit
+ * (several times as slow where not). Equal calls give equal bits; a row's last bits
+ * depend on m and on the scratch limit, which choose how its sums are split.
  * m, n and k are at most 2^22 (Resource). */
 int uocr_fp8_linear(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m, size_t k,
                     const uint8_t* w, const float* ws, size_t n, void* y, uocr_dtype ytype);
@@ -410,7 +412,7 @@ int uocr_token_logprobs_async(uocr_gpu_ctx* ctx, const void* logits, uocr_dtype 
                               size_t vocab, size_t ld, const uocr_token_scores* scores);
 /* Scores of the rows of uocr_fp8_linear's product. With n_top 0 the logits stay
  * in registers (scratch: 16 bytes per row and 128 ids, for at most 64 rows per 16
- * ids); alternatives take them through the context's scratch in f32, as many rows
+ * ids, and the copies of uocr_fp8_linear); alternatives take them through the context's scratch in f32, as many rows
  * at a time as fit (none: Resource). A row with a logit that is not finite gets
  * NaN and raises Numerical; logits in registers may do so from 1e9 on. */
 int uocr_fp8_linear_logprobs(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, size_t m,

@@ -290,9 +290,12 @@ MANY_SMALL = [(65, 33, 16), (65, 1300, 896), (100, 700, 272), (129, 2100, 1296),
               (129, 1900, 1296), (600, 500, 272)]
 # At most 64 rows of a depth that is long for its columns, and of many columns.
 FEW_DEEP = [(1, 256, 8192), (20, 512, 4096), (33, 129, 2080), (48, 2052, 2192), (64, 300, 6848), (17, 30001, 656)]
+# Rows that end anywhere: read where they are by few rows, copied for the tiles otherwise.
+RAGGED = [(1, 256, 8191), (20, 512, 4093), (48, 300, 6846), (33, 257, 1281), (100, 700, 901), (300, 1280, 2190),
+          (600, 3000, 1001), (1000, 17, 399), (64, 5000, 1279), (2, 6848, 3), (500, 900, 13)]
 
 
-@pytest.mark.parametrize("m,n,k", MANY_SMALL + FEW_DEEP)
+@pytest.mark.parametrize("m,n,k", MANY_SMALL + FEW_DEEP + RAGGED)
 def test_linear_many_rows_of_small_products(ctx, m, n, k):
     say(f"small product {m}x{n}x{k}")
     test_linear_exact(ctx, m, n, k)
@@ -356,7 +359,10 @@ def device_exact(m, n, k, seed):
                                    # More tiles than fit the card at once; depths of one, two and
                                    # many blocks, and of more than eight.
                                    (2100, 5001, 112), (1500, 6848, 272), (1300, 8000, 1296),
-                                   (130, 66000, 400), (4096, 2052, 2192)])
+                                   (130, 66000, 400), (4096, 2052, 2192),
+                                   # Rows that end anywhere.
+                                   (1, 66000, 1279), (33, 65600, 145), (64, 65537, 17), (5, 65530, 7),
+                                   (17, 70001, 1281), (2000, 6000, 1283)])
 def test_linear_wide_exact(ctx, m, n, k):
     say(f"wide product {m}x{n}x{k}")
     ops, want = device_exact(m, n, k, m + n)
@@ -391,7 +397,8 @@ def test_linear_nan_bytes_stay_in_their_row_and_column(ctx, m):
 def test_linear_depth_ends_between_rows_with_nan(ctx):
     """Rows whose bytes end inside a block: what follows in memory (the next row,
     all NaN, and bytes behind the last one) is not taken in."""
-    for m, n, k in ((3, 40, 144), (40, 300, 144), (300, 300, 130)):
+    for m, n, k in ((3, 40, 144), (40, 300, 144), (300, 300, 130), (3, 40, 133), (40, 300, 1279), (64, 5000, 1),
+                    (2, 66000, 135), (300, 1280, 2191)):
         x, xs, w, ws = exact_product(m, n, k, 5)
         x[1::2] = 0x7f
         w[1::2] = 0xff
@@ -404,10 +411,25 @@ def test_linear_depth_ends_between_rows_with_nan(ctx):
         assert np.array_equal(got, a @ b.T[:, ::2])
 
 
+@pytest.mark.parametrize("m,n,k", [(300, 700, 257), (700, 1000, 129), (200, 300, 1279), (65, 66000, 33)])
+def test_linear_without_room_for_a_copy(m, n, k):
+    """A scratch that holds neither the copy of ragged rows nor partial sums."""
+    say(f"product {m}x{n}x{k} without room")
+    cramped = um.Context(0, 4096)
+    ops, want = device_exact(m, n, k, m + k)
+    y = torch.full((m, n), float("nan"), device="cuda")
+    y16 = torch.empty((m, n), device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    um.fp8_linear(cramped, *ops, y)
+    um.fp8_linear(cramped, *ops, y16)
+    assert torch.equal(y.double(), want) and torch.equal(y16, want.float().to(torch.bfloat16))
+    cramped.close()
+
+
 def test_linear_in_a_graph_and_between_streams(ctx):
     """A captured product replays with the eager bits on what its inputs hold then;
     two contexts work at once."""
-    ops = [device_product(*random_product(m, 1000, 1280, 40 + m)) for m in (1, 30, 300)]
+    ops = [device_product(*random_product(m, 1000, k, 40 + m)) for m, k in ((1, 1280), (30, 1280), (300, 1280), (300, 1279))]
     want = []
     for d in ops:
         want.append(torch.empty((d[0].shape[0], 1000), device="cuda"))

@@ -265,7 +265,8 @@ def test_small_scratch_takes_rows_in_turn():
 # -------------------------------------------------------- from the product
 
 FUSED = [(1, 1, 16), (1, 5000, 128), (2, 63, 40), (3, 65, 1280), (7, 129, 130), (16, 1000, 256), (17, 4097, 128),
-         (40, 300, 896), (64, 257, 144), (65, 2000, 272), (130, 1537, 128), (257, 700, 384), (300, 5000, 1280)]
+         (40, 300, 896), (64, 257, 144), (65, 2000, 272), (130, 1537, 128), (257, 700, 384), (300, 5000, 1280),
+         (300, 5000, 1279), (600, 2000, 131), (40, 3001, 1)]
 
 
 def fused_reference(ops, tokens, top):
@@ -326,7 +327,8 @@ def test_linear_logprobs_many_rows_of_small_products(ctx, m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 129280, 1280), (2, 65536, 144), (19, 70001, 256), (48, 66003, 640),
-                                   (64, 65700, 2400), (1100, 8200, 272), (700, 20000, 1296)])
+                                   (64, 65700, 2400), (1100, 8200, 272), (700, 20000, 1296), (1, 66000, 1279),
+                                   (48, 66003, 641), (700, 20000, 1279)])
 def test_linear_logprobs_wide(ctx, m, n, k):
     say(f"wide fused scores {m}x{n}x{k}")
     (x, xs, w, ws), logits = device_exact(m, n, k, m + n)
@@ -401,6 +403,17 @@ def test_linear_logprobs_small_scratch():
         out = Scores(90, top)
         torch.cuda.synchronize()
         um.fp8_linear_logprobs(small, *dev, t, **out.views())
+        compare(out.host(), fused_reference(ops, tokens, top))
+        small.close()
+    # Ragged rows, with room for a copy of some of them at a time, and without.
+    ops = scaled(exact_product(300, 700, 257, 3), 2.0 ** -9)
+    tokens = np.arange(300).astype(np.int32)
+    rag, tr = device_product(*ops), torch.from_numpy(tokens).cuda()
+    for top, size in ((0, 100000), (0, 250000), (3, 120000), (3, 600000)):
+        small = um.Context(0, size)
+        out = Scores(300, top)
+        torch.cuda.synchronize()
+        um.fp8_linear_logprobs(small, *rag, tr, **out.views())
         compare(out.host(), fused_reference(ops, tokens, top))
         small.close()
     tiny = um.Context(0, 256)

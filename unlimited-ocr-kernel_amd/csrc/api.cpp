@@ -1351,7 +1351,7 @@ size_t logits_need(size_t rows, size_t vocab, const uocr_token_scores& s) {
 size_t product_need(const uocr::Fp8Product& p, size_t rows, const uocr_token_scores& s, bool pack) {
   uocr::Fp8Product q = p;
   q.m = (int)rows;
-  const size_t copy = pack ? uocr::fp8_pack_bytes(q) : 0;
+  const size_t copy = pack ? uocr::fp8_pack_bytes(q, uocr::kTypeF32, 0) : 0;
   if (copy) q.x = q.w = nullptr, q.k = (q.k + 15) / 16 * 16;  // as the copy has them
   return copy + (s.n_top ? logits_need(rows, p.n, s) : align256(uocr::fp8_score_bytes(q)));
 }
@@ -1370,7 +1370,7 @@ size_t product_rows_that_fit(size_t m, size_t limit, const Need& need, bool* pac
 // the scratch at `work` (product_need bytes).
 void enqueue_product_scores(uocr_gpu_ctx* ctx, uocr::Fp8Product p, char* work, const uocr_token_scores& s,
                             size_t row, bool pack) {
-  if (const size_t copy = pack ? uocr::fp8_pack_bytes(p) : 0) {
+  if (const size_t copy = pack ? uocr::fp8_pack_bytes(p, uocr::kTypeF32, 0) : 0) {
     p = uocr::launch_fp8_pack(p, work, ctx->stream);
     work += copy;
   }
@@ -1434,7 +1434,7 @@ int uocr_fp8_linear_async(uocr_gpu_ctx* ctx, const uint8_t* x, const float* xs, 
   uocr::Fp8Product p{x, xs, w, ws, (int)m, (int)n, (int)k};
   char* work = ctx->scratch;
   size_t bytes = ctx->scratch_limit;
-  if (const size_t copy = uocr::fp8_pack_bytes(p); copy && copy <= bytes) {
+  if (const size_t copy = uocr::fp8_pack_bytes(p, ytype, bytes); copy && copy <= bytes) {
     p = uocr::launch_fp8_pack(p, work, ctx->stream);
     work += copy;
     bytes -= copy;

@@ -195,7 +195,9 @@ void launch_fp8_quantize_tiles(const void* x, int type, int rows, int cols, size
 // 16 (more rows: more workgroups, in the grid's second dimension); KS waves of a
 // workgroup share a group's depth and add up in LDS, in order. Lane l reads the bytes
 // [16 (l / 16), +16) and 64 bytes on of row l % 16 in each block: a load instruction
-// covers 64-byte runs.
+// covers 64-byte runs. Rows that are not whole chunks (WHOLE false; the same in the kernel
+// below) are read where they are, by aligned words: 1 x 1280 x 6847 11.0 us against 7.2 at
+// 6848, 16 x 6848 x 1279 7.6 against 5.8.
 constexpr int kStreamRows = 64;
 // More than 64 rows come here only up to this many rows (whole 64) x columns x blocks.
 constexpr size_t kStreamMost = (size_t)4 << 20;
@@ -210,7 +212,7 @@ constexpr int kStreamDepth = 2;
 // x has one or two blocks of rows, 256 otherwise.
 constexpr int stream_waves(int mb) { return mb <= 2 ? 16 : 8; }
 
-template <int MB, int RG, int OUT>
+template <int MB, int RG, int OUT, bool WHOLE>
 __global__ __launch_bounds__(64 * stream_waves(MB), 2) void fp8_stream_kernel(Fp8Product p, ProductOut out,
                                                                                   StreamShape shape) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -229,6 +231,7 @@ __global__ __launch_bounds__(64 * stream_waves(MB), 2) void fp8_stream_kernel(Fp
 
   struct Stage {
     u32x4 w[RG][2], x[MB][2];
+    uint32_t w_next[WHOLE ? 1 : RG][2], x_next[WHOLE ? 1 : MB][2];
     float xs[MB], ws;
   };
   f32x4 acc[RG][MB];
@@ -240,21 +243,31 @@ __global__ __launch_bounds__(64 * stream_waves(MB), 2) void fp8_stream_kernel(Fp
   if (n0 < p.n) {
     // Rows past the last one and chunks past a row's end are out of the resources'
     // ranges: zeros, without a branch around the loads (as in the kernel below).
-    const __amdgpu_buffer_rsrc_t rw = read_rsrc(p.w + (size_t)n0 * K, (uint32_t)min(16 * RG, p.n - n0) * K);
-    const __amdgpu_buffer_rsrc_t rx = read_rsrc(p.x, (uint32_t)p.m * K);
+    const uint8_t* w0 = p.w + (size_t)n0 * K;
+    const __amdgpu_buffer_rsrc_t rw = word_rsrc<WHOLE>(w0, (uint32_t)min(16 * RG, p.n - n0) * K);
+    const __amdgpu_buffer_rsrc_t rx = word_rsrc<WHOLE>(p.x, (uint32_t)p.m * K);
+    // Where rows start, in bytes from the resources' first words.
+    const uint32_t at_w = (WHOLE ? 0 : misaligned(w0)) + (uint32_t)fr * K;
+    const uint32_t at_x = (WHOLE ? 0 : misaligned(p.x)) + (uint32_t)fr * K;
     const __amdgpu_buffer_rsrc_t rs = read_rsrc(p.xs, (uint32_t)(p.m * nkb) * 4u);
     const __amdgpu_buffer_rsrc_t rt = read_rsrc(p.ws + (size_t)(n0 / kFp8Block) * nkb, (uint32_t)nkb * 4u);
     auto load = [&](Stage& s, int kb) {
       const int k = kb * kFp8Block + 16 * fg;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        const int out_of = k + 64 * h < K ? 0 : (int)kDmaOut;  // K is a multiple of 16
+        const uint32_t out_of = k + 64 * h < K ? 0 : kDmaOut;
 #pragma unroll
-        for (int i = 0; i < RG; i++)
-          s.w[i][h] = __builtin_amdgcn_raw_buffer_load_b128(rw, ((16 * i + fr) * K + k + 64 * h) | out_of, 0, 0);
+        for (int i = 0; i < RG; i++) {
+          const uint32_t at = at_w + (uint32_t)(16 * i) * K + k + 64 * h;
+          s.w[i][h] = __builtin_amdgcn_raw_buffer_load_b128(rw, (WHOLE ? at : at & ~3u) | out_of, 0, 0);
+          if (!WHOLE) s.w_next[i][h] = __builtin_amdgcn_raw_buffer_load_b32(rw, ((at & ~3u) + 16) | out_of, 0, 0);
+        }
 #pragma unroll
-        for (int j = 0; j < MB; j++)
-          s.x[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rx, ((16 * j + fr) * K + k + 64 * h) | out_of, 0, 0);
+        for (int j = 0; j < MB; j++) {
+          const uint32_t at = at_x + (uint32_t)(16 * j) * K + k + 64 * h;
+          s.x[j][h] = __builtin_amdgcn_raw_buffer_load_b128(rx, (WHOLE ? at : at & ~3u) | out_of, 0, 0);
+          if (!WHOLE) s.x_next[j][h] = __builtin_amdgcn_raw_buffer_load_b32(rx, ((at & ~3u) + 16) | out_of, 0, 0);
+        }
       }
       const int past = kb < nkb ? 0 : (int)kDmaOut;
 #pragma unroll
@@ -263,7 +276,26 @@ __global__ __launch_bounds__(64 * stream_waves(MB), 2) void fp8_stream_kernel(Fp
             __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, ((16 * j + fr) * nkb + kb) * 4 | past, 0, 0));
       s.ws = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rt, kb * 4 | past, 0, 0));
     };
-    auto multiply = [&](const Stage& s) {
+    auto multiply = [&](Stage& s, int kb) {
+      if constexpr (!WHOLE) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+          for (int i = 0; i < RG; i++) s.w[i][h] = shift_bytes(s.w[i][h], s.w_next[i][h], at_w + 16 * i * K);
+#pragma unroll
+          for (int j = 0; j < MB; j++) s.x[j][h] = shift_bytes(s.x[j][h], s.x_next[j][h], at_x + 16 * j * K);
+        }
+        if (kb == nkb - 1) {
+          const int left = K - (kb * kFp8Block + 16 * fg);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int i = 0; i < RG; i++) s.w[i][h] = first_bytes(s.w[i][h], left - 64 * h);
+#pragma unroll
+            for (int j = 0; j < MB; j++) s.x[j][h] = first_bytes(s.x[j][h], left - 64 * h);
+          }
+        }
+      }
       bf16x8 fw[RG][4];
 #pragma unroll
       for (int i = 0; i < RG; i++)
@@ -298,7 +330,7 @@ __global__ __launch_bounds__(64 * stream_waves(MB), 2) void fp8_stream_kernel(Fp
     for (int kb = k0; kb < nkb; kb += D * shape.ks) {
 #pragma unroll
       for (int d = 0; d < D; d++) {  // those past the last block multiply zeros
-        multiply(ring[d]);
+        multiply(ring[d], kb + d * shape.ks);
         load(ring[d], kb + (d + D) * shape.ks);
       }
     }
@@ -391,7 +423,6 @@ static StreamPlan plan_stream(const Fp8Product& p, bool scores) {
 // 12.8, 64 x 1280 x 6848 19.5 and 12.7, 512 x 896 x 1280 8.7 and 11.2, 512 x 1280 x 896
 // 10.4 and 8.9, 1 x 20000 x 1280 8.8 and 10.7, 32 x 20000 x 1280 16.2 and 11.5.
 static bool takes_stream(const Fp8Product& p, int kind, size_t work_bytes) {
-  if (!whole_chunks(p)) return false;
   const size_t rows = (size_t)(p.m + kStreamRows - 1) / kStreamRows * kStreamRows;
   if (rows / kStreamRows > 65535) return false;  // a grid's second dimension
   if (p.m > kStreamRows && rows * (size_t)p.n * p.kblocks() > kStreamMost) return false;
@@ -399,28 +430,32 @@ static bool takes_stream(const Fp8Product& p, int kind, size_t work_bytes) {
   const size_t rounds = ((size_t)t.grid.x * t.grid.y + kCus - 1) / kCus;
   const size_t bytes =
       rounds * (t.shape.waves / t.shape.ks) * (16 * t.rg + std::min(p.m, kStreamRows)) * (size_t)p.k;
-  return 26 + bytes * 4e-4 <= fp8_gemm_time(p, kind != kOutBf16, work_bytes);
+  const bool whole = whole_chunks(p);
+  // The tiles' copy takes a launch, and its bytes each way at 3.3 TB/s.
+  const double copy = whole ? 0.0 : 25 + 2.0 * fp8_packed_size(p) / 3.3e5;
+  return 26 + bytes * (whole ? 4e-4 : 5e-4) <= copy + fp8_gemm_time(p, kind != kOutBf16, work_bytes);
 }
 
-template <int MB, int RG>
+template <int MB, int RG, bool WHOLE>
 static void run_stream(const Fp8Product& p, const ProductOut& out, int kind, const StreamPlan& t, hipStream_t s) {
   const dim3 grid = t.grid, block(64 * t.shape.waves);
   if (kind == kOutF32)
-    fp8_stream_kernel<MB, RG, kOutF32><<<grid, block, t.lds, s>>>(p, out, t.shape);
+    fp8_stream_kernel<MB, RG, kOutF32, WHOLE><<<grid, block, t.lds, s>>>(p, out, t.shape);
   else if (kind == kOutBf16)
-    fp8_stream_kernel<MB, RG, kOutBf16><<<grid, block, t.lds, s>>>(p, out, t.shape);
+    fp8_stream_kernel<MB, RG, kOutBf16, WHOLE><<<grid, block, t.lds, s>>>(p, out, t.shape);
   else
-    fp8_stream_kernel<MB, RG, kOutScores><<<grid, block, t.lds, s>>>(p, out, t.shape);
+    fp8_stream_kernel<MB, RG, kOutScores, WHOLE><<<grid, block, t.lds, s>>>(p, out, t.shape);
 }
+template <bool WHOLE>
 static void run_stream_rows(const Fp8Product& p, const ProductOut& out, int kind, const StreamPlan& t, hipStream_t s) {
   if (t.rg == 2) {
-    run_stream<4, 2>(p, out, kind, t, s);
+    run_stream<4, 2, WHOLE>(p, out, kind, t, s);
     return;
   }
-  if (t.mb == 1) run_stream<1, 1>(p, out, kind, t, s);
-  if (t.mb == 2) run_stream<2, 1>(p, out, kind, t, s);
-  if (t.mb == 3) run_stream<3, 1>(p, out, kind, t, s);
-  if (t.mb == 4) run_stream<4, 1>(p, out, kind, t, s);
+  if (t.mb == 1) run_stream<1, 1, WHOLE>(p, out, kind, t, s);
+  if (t.mb == 2) run_stream<2, 1, WHOLE>(p, out, kind, t, s);
+  if (t.mb == 3) run_stream<3, 1, WHOLE>(p, out, kind, t, s);
+  if (t.mb == 4) run_stream<4, 1, WHOLE>(p, out, kind, t, s);
 }
 
 // ---- few rows and many columns (a vocabulary): persistent workgroups of eight
@@ -429,7 +464,8 @@ static void run_stream_rows(const Fp8Product& p, const ProductOut& out, int kind
 // in registers until the last group: one part per workgroup and row.
 // 129280 x 1280 (165 MB), scores: one row 33 us (5.0 TB/s; the same loads alone take
 // 28.5), 48 rows 38.6 us. Four or five blocks in flight are 2 to 3 us slower, as are two
-// workgroups per CU; waves that load x from the caches instead take 39 and 66 us.
+// workgroups per CU; waves that load x from the caches instead take 39 and 66 us. With
+// 1279 columns 51 and 57 us, joins and all, against 37 and 40.
 constexpr int kWideWaves = 8, kWideDepth = 2, kWideCols = 32;
 
 struct WideShape {
@@ -442,7 +478,7 @@ static size_t wide_lds(const Fp8Product& p) {
   return rows * p.kblocks() * (kFp8Block + sizeof(float)) + kWideParts;
 }
 
-template <int MB, int OUT>
+template <int MB, int OUT, bool WHOLE>
 __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product p, ProductOut out, WideShape shape) {
   constexpr int D = kWideDepth, R = kWideCols / 16;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -456,6 +492,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
 
   struct Stage {
     u32x4 w[R][2];
+    uint32_t next[WHOLE ? 1 : R][2];
     float ws;
   };
   // Every load is issued whatever is left to do, without a branch: what lies past a
@@ -469,13 +506,17 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
   auto load = [&](Stage& s, int g, int kb) {
     const int n0 = g * kWideCols, k = kb * kFp8Block + 16 * fg;
     const int rows = g < shape.groups ? min(kWideCols, p.n - n0) : 0;
-    const __amdgpu_buffer_rsrc_t rs = read_rsrc(p.w + (size_t)n0 * K, (uint32_t)rows * K);
+    const uint8_t* w0 = p.w + (size_t)n0 * K;
+    const __amdgpu_buffer_rsrc_t rs = word_rsrc<WHOLE>(w0, (uint32_t)rows * K);
+    const uint32_t at_w = (WHOLE ? 0 : misaligned(w0)) + (uint32_t)fr * K;
 #pragma unroll
     for (int h = 0; h < 2; h++)
 #pragma unroll
-      for (int i = 0; i < R; i++)
-        s.w[i][h] = __builtin_amdgcn_raw_buffer_load_b128(
-            rs, ((16 * i + fr) * K + k + 64 * h) | (k + 64 * h < K ? 0 : (int)kDmaOut), 0, 0);
+      for (int i = 0; i < R; i++) {
+        const uint32_t at = at_w + (uint32_t)(16 * i) * K + k + 64 * h, out_of = k + 64 * h < K ? 0 : kDmaOut;
+        s.w[i][h] = __builtin_amdgcn_raw_buffer_load_b128(rs, (WHOLE ? at : at & ~3u) | out_of, 0, 0);
+        if (!WHOLE) s.next[i][h] = __builtin_amdgcn_raw_buffer_load_b32(rs, ((at & ~3u) + 16) | out_of, 0, 0);
+      }
     const int at = g < shape.groups ? ((n0 / kFp8Block) * nkb + kb) * 4 : (int)kDmaOut;
     s.ws = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rt, at, 0, 0));
   };
@@ -496,21 +537,29 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
   // The matrix's first loads are issued behind x's last ones, which return first:
   // in front of them, LDS would be filled only when the matrix has come.
   constexpr int kChunks = 3 * MB, kStep = 64 * kWideWaves;
-  const __amdgpu_buffer_rsrc_t rx = read_rsrc(p.x, (uint32_t)p.m * K);
+  const __amdgpu_buffer_rsrc_t rx = word_rsrc<WHOLE>(p.x, (uint32_t)p.m * K);
   const __amdgpu_buffer_rsrc_t rxs = read_rsrc(p.xs, (uint32_t)(p.m * nkb) * 4u);
   const int chunks = nkb * MB * 16 * 8;
   u32x4 xv[kChunks];
+  uint32_t x_next[WHOLE ? 1 : kChunks];
   auto load_x = [&](int c0) {
 #pragma unroll
     for (int i = 0; i < kChunks; i++) {
       const int c = c0 + i * kStep + tid, k = c / (MB * 16 * 8) * kFp8Block + 16 * (c & 7);
-      xv[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, (c / 8 % (MB * 16) * K + k) | (k < K ? 0 : (int)kDmaOut), 0, 0);
+      const int row = c / 8 % (MB * 16);
+      const uint32_t at = (WHOLE ? 0 : misaligned(p.x)) + (uint32_t)row * K + k, out_of = k < K ? 0 : kDmaOut;
+      xv[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, (WHOLE ? at : at & ~3u) | out_of, 0, 0);
+      if (!WHOLE) x_next[i] = __builtin_amdgcn_raw_buffer_load_b32(rx, ((at & ~3u) + 16) | out_of, 0, 0);
     }
   };
   auto store_x = [&](int c0) {
 #pragma unroll
     for (int i = 0; i < kChunks; i++) {
       const int c = c0 + i * kStep + tid, row = c / 8;
+      if constexpr (!WHOLE) {
+        const int k = c / (MB * 16 * 8) * kFp8Block + 16 * (c & 7);
+        xv[i] = first_bytes(shift_bytes(xv[i], x_next[i], misaligned(p.x) + row % (MB * 16) * K), K - k);
+      }
       if (c < chunks) *reinterpret_cast<u32x4*>(xl + (size_t)row * 128 + 16 * ((c & 7) ^ (row & 7))) = xv[i];
     }
   };
@@ -562,7 +611,19 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
   for (int at = 0; at < blocks; at += D) {
 #pragma unroll
     for (int d = 0; d < D; d++) {  // those past the last block multiply zeros
-      const Stage& s = ring[d];
+      Stage& s = ring[d];
+      if constexpr (!WHOLE) {
+        const uint32_t by = misaligned(p.w + (size_t)g * kWideCols * K) + fr * K;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int i = 0; i < R; i++) s.w[i][h] = shift_bytes(s.w[i][h], s.next[i][h], by + 16 * i * K);
+        if (kb == nkb - 1)
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < R; i++) s.w[i][h] = first_bytes(s.w[i][h], K - (kb * kFp8Block + 16 * fg + 64 * h));
+      }
       bf16x8 fw[R][4];
 #pragma unroll
       for (int i = 0; i < R; i++)
@@ -622,23 +683,34 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void fp8_wide_kernel(Fp8Product
   }
 }
 
-template <int MB>
+template <int MB, bool WHOLE>
 static void run_wide(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s) {
   const dim3 grid(kCus), block(64 * kWideWaves);
   const WideShape shape{(p.n + kWideCols - 1) / kWideCols};
   const size_t lds = wide_lds(p);
   if (kind == kOutF32)
-    fp8_wide_kernel<MB, kOutF32><<<grid, block, lds, s>>>(p, out, shape);
+    fp8_wide_kernel<MB, kOutF32, WHOLE><<<grid, block, lds, s>>>(p, out, shape);
   else if (kind == kOutBf16)
-    fp8_wide_kernel<MB, kOutBf16><<<grid, block, lds, s>>>(p, out, shape);
+    fp8_wide_kernel<MB, kOutBf16, WHOLE><<<grid, block, lds, s>>>(p, out, shape);
   else
-    fp8_wide_kernel<MB, kOutScores><<<grid, block, lds, s>>>(p, out, shape);
+    fp8_wide_kernel<MB, kOutScores, WHOLE><<<grid, block, lds, s>>>(p, out, shape);
 }
 
-template <int MB>
+template <bool WHOLE>
+static void run_wide_rows(const Fp8Product& p, const ProductOut& out, int kind, hipStream_t s) {
+  const int mb = (p.m + 15) / 16;
+  if (mb == 1) run_wide<1, WHOLE>(p, out, kind, s);
+  if (mb == 2) run_wide<2, WHOLE>(p, out, kind, s);
+  if (mb == 3) run_wide<3, WHOLE>(p, out, kind, s);
+  if (mb == 4) run_wide<4, WHOLE>(p, out, kind, s);
+}
+
+template <int MB, bool WHOLE = true>
 static void wide_attributes() {
-  const void* kernels[] = {(const void*)fp8_wide_kernel<MB, kOutF32>, (const void*)fp8_wide_kernel<MB, kOutBf16>,
-                           (const void*)fp8_wide_kernel<MB, kOutScores>};
+  if (WHOLE) wide_attributes<MB, false>();
+  const void* kernels[] = {(const void*)fp8_wide_kernel<MB, kOutF32, WHOLE>,
+                           (const void*)fp8_wide_kernel<MB, kOutBf16, WHOLE>,
+                           (const void*)fp8_wide_kernel<MB, kOutScores, WHOLE>};
   for (const void* k : kernels) (void)hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kMostLds);
 }
 void fp8_init_attributes() {
@@ -652,22 +724,24 @@ void fp8_init_attributes() {
 
 // Enough columns to keep every wave at work, and x fits into LDS.
 static bool takes_wide(const Fp8Product& p) {
-  return p.m <= kStreamRows && whole_chunks(p) && p.n >= kCus * kWideWaves * kWideCols && wide_lds(p) <= (size_t)kMostLds;
+  return p.m <= kStreamRows && p.n >= kCus * kWideWaves * kWideCols && wide_lds(p) <= (size_t)kMostLds;
 }
 
 static void launch_product(const Fp8Product& p, const ProductOut& out, int kind, void* work, size_t work_bytes,
                            hipStream_t s) {
   if (takes_wide(p)) {
-    const int mb = (p.m + 15) / 16;
-    if (mb == 1) run_wide<1>(p, out, kind, s);
-    if (mb == 2) run_wide<2>(p, out, kind, s);
-    if (mb == 3) run_wide<3>(p, out, kind, s);
-    if (mb == 4) run_wide<4>(p, out, kind, s);
+    whole_chunks(p) ? run_wide_rows<true>(p, out, kind, s) : run_wide_rows<false>(p, out, kind, s);
   } else if (takes_stream(p, kind, work_bytes)) {
-    run_stream_rows(p, out, kind, plan_stream(p, kind == kOutScores), s);
+    const StreamPlan t = plan_stream(p, kind == kOutScores);
+    whole_chunks(p) ? run_stream_rows<true>(p, out, kind, t, s) : run_stream_rows<false>(p, out, kind, t, s);
   } else {
     launch_fp8_gemm(p, out, kind, work, work_bytes, s);
   }
+}
+
+size_t fp8_pack_bytes(const Fp8Product& p, int ytype, size_t work_bytes) {
+  if (whole_chunks(p) || takes_wide(p) || takes_stream(p, ytype == kTypeF32 ? kOutF32 : kOutBf16, work_bytes)) return 0;
+  return fp8_packed_size(p);
 }
 
 void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, void* work, size_t work_bytes, hipStream_t s) {

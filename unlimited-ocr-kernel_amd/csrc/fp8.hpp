@@ -33,10 +33,12 @@ struct Fp8Product {
   int m, n, k;
   __host__ __device__ int kblocks() const { return (k + kFp8Block - 1) / kFp8Block; }
 };
-// Rows of whole 16-byte chunks at aligned addresses, which the fast kernels take. Where p's
-// are not, a copy of both operands that are, with zeros behind each row's end: its bytes
-// (0 where it needs none), and the launch that makes it at `work` (256-byte aligned).
-size_t fp8_pack_bytes(const Fp8Product& p);
+// Tiles are staged from rows of whole 16-byte chunks at aligned addresses. Where p's are
+// not and tiles are what takes it, a copy of both operands that are, with zeros behind each
+// row's end: its bytes (0 where it needs none), and the launch that makes it at `work`
+// (256-byte aligned). ytype and work_bytes are those of the launch below; scores, kTypeF32
+// and 0.
+size_t fp8_pack_bytes(const Fp8Product& p, int ytype, size_t work_bytes);
 Fp8Product launch_fp8_pack(const Fp8Product& p, void* work, hipStream_t s);
 // `work`: room for partial sums where the depth is split; any size will do.
 void launch_fp8_linear(const Fp8Product& p, void* y, int ytype, void* work, size_t work_bytes, hipStream_t s);

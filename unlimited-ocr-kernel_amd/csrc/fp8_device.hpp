@@ -128,6 +128,35 @@ void fp8_gemm_init_attributes();
 // The launch's modelled time in units of 0.1 us (whole_chunks only).
 double fp8_gemm_time(const Fp8Product& p, bool widen, size_t work_bytes);
 
+// Rows at any address are read by aligned words, one more than the bytes wanted, and moved
+// to their places (loads at addresses that are no multiple of 4 take some three times as
+// long). A resource of `bytes` bytes from p on then starts at p's word and ends with the
+// last byte's.
+__device__ __forceinline__ uint32_t misaligned(const uint8_t* p) { return (uint32_t)reinterpret_cast<uintptr_t>(p) & 3; }
+template <bool WHOLE>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t word_rsrc(const uint8_t* p, uint32_t bytes) {
+  if (WHOLE) return read_rsrc(p, bytes);
+  const uint32_t by = misaligned(p);
+  return read_rsrc(p - by, (bytes + by + 3) & ~3u);
+}
+__device__ __forceinline__ u32x4 shift_bytes(u32x4 v, uint32_t next, uint32_t by) {
+  by &= 3;
+  return (u32x4){__builtin_amdgcn_alignbyte(v.y, v.x, by), __builtin_amdgcn_alignbyte(v.z, v.y, by),
+                 __builtin_amdgcn_alignbyte(v.w, v.z, by), __builtin_amdgcn_alignbyte(next, v.w, by)};
+}
+// The first `left` bytes, zeros behind them.
+__device__ __forceinline__ u32x4 first_bytes(u32x4 v, int left) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int bits = min(max(left - 4 * i, 0), 4) * 8;
+    v[i] = bits == 32 ? v[i] : v[i] & ((1u << bits) - 1);
+  }
+  return v;
+}
+
+// Bytes of fp8_pack_bytes' copy.
+size_t fp8_packed_size(const Fp8Product& p);
+
 // Whole 16-byte chunks of rows at aligned addresses.
 inline bool whole_chunks(const Fp8Product& p) {
   return p.k % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0;

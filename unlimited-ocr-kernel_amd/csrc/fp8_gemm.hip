@@ -5,24 +5,28 @@
 
 namespace uocr {
 
-// Sixteen bytes of a row of K bytes from byte k, zeros behind the row's end.
-// Rows start at any address where K is not a multiple of 16.
+// Sixteen bytes of a row of K bytes from byte k, zeros behind the row's end, of rows that
+// start at any address: by the aligned words that hold any of them.
 __device__ __forceinline__ uint4 load_chunk(const uint8_t* row, int k, int K) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (k + 16 <= K) {
-    __builtin_memcpy(&v, row + k, 16);
+  if (k >= K) return make_uint4(0, 0, 0, 0);
+  const int left = min(K - k, 16), by = (int)misaligned(row + k);
+  const auto* at = reinterpret_cast<const uint32_t*>(row + k - by);
+  const int words = (by + left + 3) / 4;
+  u32x4 v = {0, 0, 0, 0};
+  if (words >= 4) {
+    __builtin_memcpy(&v, __builtin_assume_aligned(at, 4), 16);
   } else {
-    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < 16; j++)
-      if (k + j < K) w[j / 4] |= (uint32_t)row[k + j] << (8 * (j & 3));
-    v = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 3; i++)
+      if (i < words) v[i] = at[i];
   }
-  return v;
+  v = first_bytes(shift_bytes(v, words == 5 ? at[4] : 0, by), left);
+  return make_uint4(v.x, v.y, v.z, v.w);
 }
 
 // Both operands with rows of whole chunks, a chunk per thread. 4096 x 6848 x 1279 f32:
-// 219 us on the kernel below, 102 on tiles of such a copy; 1 x 1280 x 6847 142 and 14.
+// 219 us on the kernel below, 99 with such a copy and its tiles; 277 x 1280 x 6847 194 and
+// 26.
 __global__ __launch_bounds__(256) void fp8_pack_kernel(Fp8Product p, uint8_t* __restrict__ x, uint8_t* __restrict__ w) {
   const uint32_t chunks = (p.k + 15) / 16, all_x = p.m * chunks, all = all_x + p.n * chunks;
   uint32_t c = blockIdx.x * 256 + threadIdx.x;
@@ -36,8 +40,7 @@ __global__ __launch_bounds__(256) void fp8_pack_kernel(Fp8Product p, uint8_t* __
 // A thread per chunk, counted in 32 bits: larger copies have no room anywhere.
 constexpr size_t kMostPacked = (size_t)1 << 35;
 static size_t pack_part(int rows, int k) { return ((size_t)rows * ((k + 15) / 16) * 16 + 255) / 256 * 256; }
-size_t fp8_pack_bytes(const Fp8Product& p) {
-  if (whole_chunks(p)) return 0;
+size_t fp8_packed_size(const Fp8Product& p) {
   const size_t bytes = pack_part(p.m, p.k) + pack_part(p.n, p.k);
   return bytes < kMostPacked ? bytes : SIZE_MAX / 2;
 }
