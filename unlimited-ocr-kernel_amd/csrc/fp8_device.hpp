@@ -132,7 +132,7 @@ double fp8_gemm_time(const Fp8Product& p, bool widen, size_t work_bytes);
 // to their places (loads at addresses that are no multiple of 4 take some three times as
 // long). A resource of `bytes` bytes from p on then starts at p's word and ends with the
 // last byte's.
-__device__ __forceinline__ uint32_t misaligned(const uint8_t* p) { return (uint32_t)reinterpret_cast<uintptr_t>(p) & 3; }
+__device__ __forceinline__ uint32_t misaligned(const void* p) { return (uint32_t)reinterpret_cast<uintptr_t>(p) & 3; }
 template <bool WHOLE>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t word_rsrc(const uint8_t* p, uint32_t bytes) {
   if (WHOLE) return read_rsrc(p, bytes);
