@@ -131,13 +131,13 @@ double fp8_gemm_time(const Fp8Product& p, bool widen, size_t work_bytes);
 // Rows at any address are read by aligned words, one more than the bytes wanted, and moved
 // to their places (loads at addresses that are no multiple of 4 take some three times as
 // long). A resource of `bytes` bytes from p on then starts at p's word and ends with the
-// last byte's.
+// last byte's; each word of a 16-byte load is checked for itself.
 __device__ __forceinline__ uint32_t misaligned(const void* p) { return (uint32_t)reinterpret_cast<uintptr_t>(p) & 3; }
 template <bool WHOLE>
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t word_rsrc(const uint8_t* p, uint32_t bytes) {
   if (WHOLE) return read_rsrc(p, bytes);
   const uint32_t by = misaligned(p);
-  return read_rsrc(p - by, (bytes + by + 3) & ~3u);
+  return read_rsrc(p - by, bytes ? (bytes + by + 3) & ~3u : 0);  // no byte, no word
 }
 __device__ __forceinline__ u32x4 shift_bytes(u32x4 v, uint32_t next, uint32_t by) {
   by &= 3;
