@@ -8,6 +8,7 @@
 namespace uocr {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // A raw buffer resource for loads: those at or past `bytes` give zeros.
@@ -61,11 +62,11 @@ __device__ __forceinline__ void store_columns(const Fp8Product& p, void* y, int 
   }
 }
 
-// The statistics of one row's logits in a wave: lane l holds columns col + 16 i +
-// r of row l % 16 (v[i][r]; col differs by 4 between the four lanes of a row). Every
-// lane of the row gets them. The lane with the given token's column keeps its logit.
-// FULL: all of the columns are below n.
-template <int COUNT, bool FULL>
+// The statistics of one row's logits in a wave: lane l holds columns col + STRIDE i +
+// r of row l % 16 (v[i][r]; col differs by 4 between the four lanes of a row) or, with a
+// STRIDE of 8, of row l % 32 (two lanes). Every lane of the row gets them. The lane with
+// the given token's column keeps its logit. FULL: all of the columns are below n.
+template <int COUNT, bool FULL, int STRIDE>
 __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int col, int n, int token,
                                                     float* given) {
   ScorePart q = empty_part();
@@ -73,8 +74,8 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
 #pragma unroll
   for (int i = 0; i < COUNT; i++)
 #pragma unroll
-    for (int r = 0; r < 4; r++) most = FULL || col + 16 * i + r < n ? fmaxf(most, v[i][r]) : most;
-  most = fmaxf(most, __shfl_xor(most, 16));
+    for (int r = 0; r < 4; r++) most = FULL || col + STRIDE * i + r < n ? fmaxf(most, v[i][r]) : most;
+  if (STRIDE == 16) most = fmaxf(most, __shfl_xor(most, 16));
   most = fmaxf(most, __shfl_xor(most, 32));
   // d = log2(e) x - r2 in one instruction; r2's rounding c, the same for all of the
   // row's logits here, is put right at the end: the terms are 2^(d + c). Beyond 1e9 c is
@@ -85,22 +86,22 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
   for (int i = 0; i < COUNT; i++)
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const float d = FULL || col + 16 * i + r < n ? fmaf(v[i][r], kLog2e, -r2) : -1000.0f;
+      const float d = FULL || col + STRIDE * i + r < n ? fmaf(v[i][r], kLog2e, -r2) : -1000.0f;
       const float e = __builtin_amdgcn_exp2f(d);
       q.s += e;
       q.t = fmaf(e, d, q.t);
     }
   const uint32_t off = (uint32_t)(token - col);
-  if (off < 16u * COUNT && (off & 12u) == 0 && token < n) {
+  if (off < (uint32_t)STRIDE * COUNT && (off & (STRIDE - 4u)) == 0 && token < n) {
     float g = 0.0f;
 #pragma unroll
     for (int i = 0; i < COUNT; i++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) g = off == 16u * i + r ? v[i][r] : g;
+      for (int r = 0; r < 4; r++) g = off == (uint32_t)STRIDE * i + r ? v[i][r] : g;
     *given = g;
   }
 #pragma unroll
-  for (int o = 16; o <= 32; o <<= 1) {
+  for (int o = STRIDE == 16 ? 16 : 32; o <= 32; o <<= 1) {
     q.s += __shfl_xor(q.s, o);
     q.t += __shfl_xor(q.t, o);
   }
@@ -111,11 +112,11 @@ __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int
   return q;
 }
 // The same, whether or not the wave's columns (from n0 on) end below n.
-template <int COUNT>
+template <int COUNT, int STRIDE = 16>
 __device__ __forceinline__ ScorePart row_statistics(const f32x4 (&v)[COUNT], int n0, int fg, int n, int token,
                                                     float* given) {
-  return n0 + 16 * COUNT <= n ? row_statistics<COUNT, true>(v, n0 + 4 * fg, n, token, given)
-                              : row_statistics<COUNT, false>(v, n0 + 4 * fg, n, token, given);
+  return n0 + STRIDE * COUNT <= n ? row_statistics<COUNT, true, STRIDE>(v, n0 + 4 * fg, n, token, given)
+                                  : row_statistics<COUNT, false, STRIDE>(v, n0 + 4 * fg, n, token, given);
 }
 
 // fp8_gemm.hip: the product of many rows.

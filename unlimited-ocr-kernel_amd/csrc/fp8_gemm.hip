@@ -138,14 +138,16 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 // 64 x 64 or 32 x 64 each. A stage is one scale block deep: the tile's rows and columns,
 // 128 bytes of each, brought by global->LDS loads into a ring of buffers ahead of the one
 // that is multiplied. The matrix is the matrix instruction's first operand: lane l then
-// holds four adjacent columns of y for row l % 16, whose x scale it needs as one value.
+// holds groups of four adjacent columns of y for one row of x, whose scale it needs as one
+// value.
 //
 // WIDEN: the matrix cores' e4m3 instructions bring each group of eight products to
 // the largest one's exponent and cut them off 13 bits below it (measured: 2^16 -
 // 2^16 + v keeps multiples of 8; 1.3e-5 of a Gaussian block's sum). Results in f32
 // and scores widen the operands to bf16 instead, whose products are summed to f32's
-// last bit (1e-8): a scale block is a chain of four v_mfma_f32_16x16x32_bf16 from
-// zero. bf16 results, rounded to 2^-9 anyway, take v_mfma_f32_16x16x128_f8f6f4, one
+// last bit (1e-8): a scale block is a chain of eight v_mfma_f32_32x32x16_bf16 from zero
+// (four v_mfma_f32_16x16x32_bf16 are twice the instructions to issue: 277 x 1280 x 6848
+// 16.4 -> 15.8 us, 100 x 20000 x 1280 scores 16.0 -> 14.2). bf16 results, rounded to 2^-9 anyway, take v_mfma_f32_16x16x128_f8f6f4, one
 // per scale block, at twice the rate. Either way a block's sum is scaled into the f32
 // accumulators when it is done.
 //
@@ -161,9 +163,10 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 // launch adds them in order.
 //
 // 4096 x 6848 x 1280 bf16 55 us (1310 TFLOP/s): the loads bring 17 TB/s into LDS, which is
-// what bounds the steps, and the stores take 10 us. 4096 x 129280 x 1280 scores 1275 us
-// (1060 TFLOP/s): the vector instructions, 3.4 a product (2 of widening, 1 of scaling) and
-// the statistics', share the issue with the products.
+// what bounds the steps, and the stores take 10 us. 4096 x 129280 x 1280 scores 1264 us
+// (1070 TFLOP/s): the vector instructions, 3.4 to 16 x 16 x 32 products (2 of widening, 1 of
+// scaling), and
+// the statistics' share the issue with the products.
 constexpr int kCols = 128;  // columns of a tile
 constexpr int short_bufs(bool widen) { return widen ? 2 : 3; }
 constexpr int short_per_cu(bool widen) { return widen ? 3 : 2; }
@@ -194,6 +197,11 @@ __device__ __forceinline__ TileAt tile_of(int id, int tiles_m, int tiles_n) {
 struct Splits {
   int count, each;
 };
+
+// Four adjacent columns of a 32 x 32 block's sixteen.
+__device__ __forceinline__ f32x4 quarter(const f32x16& v, int i) {
+  return (f32x4){v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+}
 
 template <bool WIDEN, int OUT, int BUFS, int XB>
 __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductOut out, Splits splits) {
@@ -257,72 +265,94 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
     if (tid < 8) to[8 * kRows + tid] = __uint_as_float(s.w);
   };
 
+  // WIDEN: blocks of 32 x 32 (twice XB / 2 of them in a wave), whose lane l has row l % 32
+  // of x and columns 8 i + 4 (l / 32) + r; otherwise of 16 x 16.
+  constexpr int JB = XB / 2;
+  const int r32 = lane & 31, half = lane >> 5;
   f32x4 acc[4][XB];
+  f32x16 wide[2][JB];
 #pragma unroll
   for (int i = 0; i < 4; i++)
 #pragma unroll
     for (int j = 0; j < XB; j++) acc[i][j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < JB; j++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) wide[i][j][r] = 0.0f;
   auto chunk_at = [&](const char* tile, int r, int c) {
     return *reinterpret_cast<const u32x4*>(tile + r * 128 + 16 * (c ^ (r & 7)));
   };
-  // Lane group g takes chunks g and g + 4 of both operands: the order of the 128
-  // products inside a block is free.
-  struct Raw {
-    u32x4 half[2];
-  };
-  auto read = [&](const char* tile, int r) { return Raw{{chunk_at(tile, r, fg), chunk_at(tile, r, fg + 4)}}; };
-  // One stage. While row block j is multiplied, block j - 1's sums are scaled, block
-  // j + 1's fragment is widened and block j + 2's is read; the order within a step is
-  // held by sched_barrier. Left to itself the compiler waits for each product before
-  // it scales it.
-  auto scale = [&](f32x4& a, const f32x4& d, float sc) {
-#pragma unroll
-    for (int r = 0; r < 4; r++) a[r] = fmaf(d[r], sc, a[r]);
-    asm volatile("" : "+v"(a));  // here, not sunk behind the loop's next branch
-  };
+  // One stage. The order of the 128 products inside a block is free, so lanes take whole
+  // chunks of their rows. What stands between products is held there by sched_barrier:
+  // left to itself the compiler waits for each product before it scales it.
   auto multiply = [&](int kb) {
     const char* xt = lds + (size_t)(kb % BUFS) * kStage;
     const char* wt = xt + kRows * 128;
-    const float* xs = scales_at(kb >> 3) + (kb & 7) * kRows + wm + fr;
+    const float* xs = scales_at(kb >> 3) + (kb & 7) * kRows + wm;
     const float ws = scales_at(kb >> 3)[8 * kRows + (kb & 7)];
-    float sc[2];
-    f32x4 d[2][4];
-    auto zero = [&](f32x4 (&v)[4]) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    };
     if constexpr (WIDEN) {
-      // Eight values of a fragment: half h / 2's words 2 (h % 2) and 2 (h % 2) + 1.
-      auto part = [&](const Raw& v, int h) { return widen_fp8x8(v.half[h / 2][2 * (h & 1)], v.half[h / 2][2 * (h & 1) + 1]); };
-      Raw rw4[4], raw[2];
-      bf16x8 fw[4][4], fx[2][4];
-      raw[0] = read(xt, wm + fr);
+      // Lane half g takes chunks 4 g to 4 g + 3, eight bytes to a product; the operands
+      // of the next eight are widened under the products of these.
+      u32x4 w4[2][4], x4[JB][4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) rw4[i] = read(wt, wn + 16 * i + fr);
-      if (XB > 1) raw[1] = read(xt, wm + 16 + fr);
+      for (int t = 0; t < 4; t++) {
 #pragma unroll
-      for (int h = 0; h < 4; h++) fx[0][h] = part(raw[0], h);
+        for (int j = 0; j < JB; j++) x4[j][t] = chunk_at(xt, wm + 32 * j + r32, 4 * half + t);
 #pragma unroll
-      for (int h = 0; h < 4; h++)
+        for (int i = 0; i < 2; i++) w4[i][t] = chunk_at(wt, wn + 32 * i + r32, 4 * half + t);
+      }
+      float sc[JB];
 #pragma unroll
-        for (int i = 0; i < 4; i++) fw[i][h] = part(rw4[i], h);
+      for (int j = 0; j < JB; j++) sc[j] = xs[32 * j + r32] * ws;
+      auto part = [&](const u32x4 (&v)[4], int u) { return widen_fp8x8(v[u / 2][2 * (u & 1)], v[u / 2][2 * (u & 1) + 1]); };
+      bf16x8 fw[2][2], fx[2][JB];
+      f32x16 d[2][JB];
+#pragma unroll
+      for (int j = 0; j < JB; j++) fx[0][j] = part(x4[j], 0);
+#pragma unroll
+      for (int i = 0; i < 2; i++) fw[0][i] = part(w4[i], 0);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int j = 0; j < XB; j++) {
-        if (j + 2 < XB) raw[j & 1] = read(xt, wm + 16 * (j + 2) + fr);
-        sc[j & 1] = xs[16 * j] * ws;
-        zero(d[j & 1]);
+      for (int u = 0; u < 8; u++) {
 #pragma unroll
-        for (int h = 0; h < 4; h++) {
+        for (int j = 0; j < JB; j++)
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            d[j & 1][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[i][h], fx[j & 1][h], d[j & 1][i], 0, 0, 0);
-          if (j + 1 < XB) fx[(j + 1) & 1][h] = part(raw[(j + 1) & 1], h);
-          if (j > 0) scale(acc[h][j - 1], d[(j - 1) & 1][h], sc[(j - 1) & 1]);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+          for (int i = 0; i < 2; i++) {
+            if (u == 0)
+#pragma unroll
+              for (int r = 0; r < 16; r++) d[i][j][r] = 0.0f;
+            d[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw[u & 1][i], fx[u & 1][j], d[i][j], 0, 0, 0);
+            if (u < 7) {
+              if (j == 0) fw[(u + 1) & 1][i] = part(w4[i], u + 1);
+              if (j == JB - 1 && i < JB) fx[(u + 1) & 1][i] = part(x4[i], u + 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
       }
+#pragma unroll
+      for (int j = 0; j < JB; j++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+#pragma unroll
+          for (int r = 0; r < 16; r++) wide[i][j][r] = fmaf(d[i][j][r], sc[j], wide[i][j][r]);
+          asm volatile("" : "+v"(wide[i][j]));  // here, not sunk behind the loop's next branch
+        }
     } else {
+      // Lane group g takes chunks g and g + 4. While row block j is multiplied, block j - 1's
+      // sums are scaled and block j + 1's fragment is read.
+      struct Raw {
+        u32x4 half[2];
+      };
+      auto read = [&](const char* tile, int r) { return Raw{{chunk_at(tile, r, fg), chunk_at(tile, r, fg + 4)}}; };
+      auto scale = [&](f32x4& a, const f32x4& d, float sc) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) a[r] = fmaf(d[r], sc, a[r]);
+        asm volatile("" : "+v"(a));
+      };
+      float sc[2];
+      f32x4 d[2][4];
       auto whole = [&](const Raw& v) {
         return (i32x8){(int)v.half[0].x, (int)v.half[0].y, (int)v.half[0].z, (int)v.half[0].w,
                        (int)v.half[1].x, (int)v.half[1].y, (int)v.half[1].z, (int)v.half[1].w};
@@ -335,19 +365,19 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
 #pragma unroll
       for (int j = 0; j < XB; j++) {
         if (j + 1 < XB) fx[(j + 1) & 1] = read(xt, wm + 16 * (j + 1) + fr);
-        sc[j & 1] = xs[16 * j] * ws;
-        zero(d[j & 1]);
+        sc[j & 1] = xs[16 * j + fr] * ws;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          d[j & 1][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(whole(fw[i]), whole(fx[j & 1]), d[j & 1][i], 0,
-                                                                         0, 0, 0, 0, 0);
+          const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+          d[j & 1][i] =
+              __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(whole(fw[i]), whole(fx[j & 1]), zero, 0, 0, 0, 0, 0, 0);
           if (j > 0) scale(acc[i][j - 1], d[(j - 1) & 1][i], sc[(j - 1) & 1]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; i++) scale(acc[i][XB - 1], d[(XB - 1) & 1][i], sc[(XB - 1) & 1]);
+      for (int i = 0; i < 4; i++) scale(acc[i][XB - 1], d[(XB - 1) & 1][i], sc[(XB - 1) & 1]);
+    }
   };
 
   // Stage kb is multiplied while the BUFS - 1 behind it are on their way. A wave's loads
@@ -382,19 +412,29 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
     ScorePart* held = reinterpret_cast<ScorePart*>(lds);
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < XB; j++) {
-      const int r = wm + 16 * j + fr, row = m0 + r;
+    for (int j = 0; j < JB; j++) {
+      const int r = wm + 32 * j + r32, row = m0 + r;
       const int token = out.tokens && row < p.m ? out.tokens[row] : -1;
-      const f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+      f32x4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) v[i] = quarter(wide[i / 4][j], i % 4);
       ScorePart q = empty_part();
-      if (n0 + wn < p.n) q = row_statistics<4>(v, n0 + wn, fg, p.n, token, out.given + row);
-      if (fg == 0) held[wave % 2 * kRows + r] = q;
+      if (n0 + wn < p.n) q = row_statistics<8, 8>(v, n0 + wn, half, p.n, token, out.given + row);
+      if (half == 0) held[wave % 2 * kRows + r] = q;
     }
     __syncthreads();
     if (tid < kRows && m0 + tid < p.m)
       out.parts[(size_t)tile.n * p.m + m0 + tid] = join(held[tid], held[kRows + tid]);
   } else {
     char* y = static_cast<char*>(out.y) + (size_t)split * p.m * p.n * (OUT == kOutF32 ? 4 : 2);
+    if constexpr (WIDEN) {
+#pragma unroll
+      for (int j = 0; j < JB; j++)
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          store_columns<OUT>(p, y, m0 + wm + 32 * j + r32, n0 + wn + 8 * i + 4 * half, quarter(wide[i / 4][j], i % 4));
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < XB; j++)
 #pragma unroll
