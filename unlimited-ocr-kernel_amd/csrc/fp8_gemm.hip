@@ -164,9 +164,8 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 //
 // 4096 x 6848 x 1280 bf16 55 us (1310 TFLOP/s): the loads bring 17 TB/s into LDS, which is
 // what bounds the steps, and the stores take 10 us. 4096 x 129280 x 1280 scores 1264 us
-// (1070 TFLOP/s): the vector instructions, 3.4 to 16 x 16 x 32 products (2 of widening, 1 of
-// scaling), and
-// the statistics' share the issue with the products.
+// (1070 TFLOP/s): the vector instructions (3.4 to 16 x 16 x 32 products, of them 2 of
+// widening and 1 of scaling, and the statistics') share the issue with the products.
 constexpr int kCols = 128;  // columns of a tile
 constexpr int short_bufs(bool widen) { return widen ? 2 : 3; }
 constexpr int short_per_cu(bool widen) { return widen ? 3 : 2; }
