@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 // and scores widen the operands to bf16 instead, whose products are summed to f32's
 // last bit (1e-8): a scale block is a chain of eight v_mfma_f32_32x32x16_bf16 from zero
 // (four v_mfma_f32_16x16x32_bf16 are twice the instructions to issue: 277 x 1280 x 6848
-// 16.4 -> 15.8 us, 100 x 20000 x 1280 scores 16.0 -> 14.2). bf16 results, rounded to 2^-9 anyway, take v_mfma_f32_16x16x128_f8f6f4, one
+// 16.4 -> 15.6 us, 100 x 20000 x 1280 scores 16.0 -> 14.2). bf16 results, rounded to 2^-9 anyway, take v_mfma_f32_16x16x128_f8f6f4, one
 // per scale block, at twice the rate. Either way a block's sum is scaled into the f32
 // accumulators when it is done.
 //
@@ -163,8 +163,8 @@ __global__ __launch_bounds__(256) void fp8_bytes_kernel(Fp8Product p, ProductOut
 // launch adds them in order.
 //
 // 4096 x 6848 x 1280 bf16 55 us (1310 TFLOP/s): the loads bring 17 TB/s into LDS, which is
-// what bounds the steps, and the stores take 10 us. 4096 x 129280 x 1280 scores 1264 us
-// (1070 TFLOP/s): the vector instructions (3.4 to 16 x 16 x 32 products, of them 2 of
+// what bounds the steps, and the stores take 10 us. 4096 x 129280 x 1280 scores 1246 us
+// (1090 TFLOP/s): the vector instructions (3.4 to 16 x 16 x 32 products, of them 2 of
 // widening and 1 of scaling, and the statistics') share the issue with the products.
 constexpr int kCols = 128;  // columns of a tile
 constexpr int short_bufs(bool widen) { return widen ? 2 : 3; }
@@ -220,24 +220,28 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
   const int wm = wave / 2 * (16 * XB), wn = wave % 2 * 64;
 
   // Loads: a wave instruction brings 8 rows of 128 bytes; chunk c of row r lies at c
-  // ^ (r % 8), which spreads a fragment read's sixteen rows over all banks.
+  // ^ (r / 2 % 8), which spreads a fragment read's rows, sixteen of two chunks or 32 of
+  // one, over all banks (two rows fill them).
   constexpr int kSegsX = kRows / 8 / 4, kSegsW = kCols / 8 / 4, kLoads = kSegsX + kSegsW;
   const i32x4 rx = buffer_rsrc(p.x + (size_t)m0 * K, (uint32_t)min(kRows, p.m - m0) * K);
   const i32x4 rw = buffer_rsrc(p.w + (size_t)n0 * K, (uint32_t)min(kCols, p.n - n0) * K);
-  const int chunk = (lane & 7) ^ (lane >> 3);
-  const uint32_t at_x = (uint32_t)(wave * kSegsX * 8 + (lane >> 3)) * K + 16 * chunk;
-  const uint32_t at_w = (uint32_t)(wave * kSegsW * 8 + (lane >> 3)) * K + 16 * chunk;
+  static_assert(kSegsX % 2 == 0 && kSegsW % 2 == 0, "a wave's first rows are a multiple of 16");
+  const uint32_t chunk[2] = {(uint32_t)((lane & 7) ^ (lane >> 4)) * 16, (uint32_t)((lane & 7) ^ (lane >> 4) ^ 4) * 16};
+  const uint32_t at_x = (uint32_t)(wave * kSegsX * 8 + (lane >> 3)) * K;
+  const uint32_t at_w = (uint32_t)(wave * kSegsW * 8 + (lane >> 3)) * K;
   const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds);
   auto issue = [&](int kb) {
     const uint32_t k = (uint32_t)kb * 128u;
-    const uint32_t past = (int)k + 16 * chunk < K ? 0u : kDmaOut;
+    uint32_t at[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) at[i] = (k + chunk[i]) | ((int)(k + chunk[i]) < K ? 0u : kDmaOut);
     const uint32_t to = __builtin_amdgcn_readfirstlane(lds0 + (uint32_t)(kb % BUFS) * kStage);
 #pragma unroll
     for (int i = 0; i < kSegsW; i++) {
       if (i < kSegsX)
-        buffer_load_lds16(rx, to + (uint32_t)(wave * kSegsX + i) * 1024u, (at_x + (uint32_t)(8 * i) * K + k) | past);
+        buffer_load_lds16(rx, to + (uint32_t)(wave * kSegsX + i) * 1024u, at_x + (uint32_t)(8 * i) * K + at[i & 1]);
       buffer_load_lds16(rw, to + kRows * 128u + (uint32_t)(wave * kSegsW + i) * 1024u,
-                        (at_w + (uint32_t)(8 * i) * K + k) | past);
+                        at_w + (uint32_t)(8 * i) * K + at[i & 1]);
     }
   };
   // Scales of eight blocks at a time, in LDS beside the stages. A thread brings four
@@ -281,7 +285,7 @@ __global__ __launch_bounds__(256, 2) void fp8_tile_kernel(Fp8Product p, ProductO
 #pragma unroll
       for (int r = 0; r < 16; r++) wide[i][j][r] = 0.0f;
   auto chunk_at = [&](const char* tile, int r, int c) {
-    return *reinterpret_cast<const u32x4*>(tile + r * 128 + 16 * (c ^ (r & 7)));
+    return *reinterpret_cast<const u32x4*>(tile + r * 128 + 16 * (c ^ (r / 2 & 7)));
   };
   // One stage. The order of the 128 products inside a block is free, so lanes take whole
   // chunks of their rows. What stands between products is held there by sched_barrier:
